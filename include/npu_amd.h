@@ -392,6 +392,146 @@ int gm_rms_norm(const float* x, const float* w, int D, int n_rows, float eps, fl
  */
 int gm_moe_forward_noalloc(const gm_moe_layer* L, const float* x, float* y, int T, int flags, void* stream);
 
+/*
+ * Serving a batch of sequences: positions with several axes, a key-value cache
+ * in pages, attention over it, and sampling.  The reference runs one sequence
+ * with one position per token (qwen/forward.py:64-97), grows one cache by
+ * concatenation (:133-239) and returns logits (:834-893); these are the same
+ * steps for many sequences at once.
+ *
+ * Element types are GM_QTYPE_F32, GM_QTYPE_F16 or GM_QTYPE_BF16.  Strides are in
+ * elements; a row of head_dim elements is contiguous.  A cache is two arrays
+ * [n_pages][page_size][n_head_kv][head_dim] (k and v) of F16 or BF16, 16-byte
+ * aligned; a block table [n_seq][table_width] int32 holds the page numbers of
+ * each sequence in order.  A page number outside [0, n_pages) holds no keys: its
+ * positions are masked.  head_dim is 64, 128 or 256; n_head a multiple of
+ * n_head_kv, scale positive.  Every length, offset and table is read on the device
+ * only.
+ */
+
+/*
+ * q_out = rot(rmsnorm(q) q_norm), and rot(rmsnorm(k) k_norm) and v to the
+ * cache's row slots[t] (page number times page_size plus the row in the page; one
+ * outside [0, n_rows) writes nothing; a slot given twice keeps either row).
+ * rot turns the pairs (i, i + rope_dim / 2) by positions[axis[i]][t] * inv_freq[i]
+ * radians, formed in 64 bits; dims from rope_dim on are not turned.  rope_dim is
+ * even and at most head_dim.  The norms are left out where q_norm / k_norm is NULL.
+ * Replaces qwen/forward.py:81-97, :179-199 for many sequences.
+ */
+typedef struct gm_rope_append_args {
+  const void* q;             /* [T][n_head][head_dim] in in_type, strides below */
+  const void* k;             /* [T][n_head_kv][head_dim] */
+  const void* v;
+  const int32_t* positions;  /* [n_axes][T] */
+  const double* inv_freq;    /* [rope_dim / 2] radians per position */
+  const int32_t* axis;       /* [rope_dim / 2], each 0 .. n_axes - 1 (others count as 0); NULL: axis 0 */
+  const float* q_norm;       /* [head_dim] or NULL */
+  const float* k_norm;       /* [head_dim] or NULL */
+  void* q_out;               /* [T][n_head][head_dim] in out_type, contiguous, 16-byte aligned */
+  void* k_pages;             /* n_rows rows of [n_head_kv][head_dim] in cache_type */
+  void* v_pages;
+  const int32_t* slots;      /* [T] */
+  int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h;
+  int64_t v_stride_t, v_stride_h;
+  int64_t n_rows;            /* n_pages page_size */
+  float eps;
+  int32_t T, n_axes, n_head, n_head_kv;
+  int32_t head_dim, rope_dim;
+  int32_t in_type, out_type, cache_type;
+} gm_rope_append_args;
+int gm_rope_append(const gm_rope_append_args* a, void* stream);
+
+/*
+ * Attention of one new token per sequence over the cache:
+ * out[b][h] = softmax(scale q[b][h] . K) V (times sigmoid(gate[b][h])) over
+ * positions 0 .. lengths[b] - 1 (the new token's own row among them, written
+ * before), query head h reading kv head h / (n_head / n_head_kv).  Zeros where a
+ * sequence has no key (length <= 0); lengths past table_width * page_size count
+ * as that.  q and out are F32 (any cache type) or the cache's type.  n_seq is at
+ * most 8192.  Work is split over the lengths and joined by a second launch;
+ * partial results are in the workspace, and no result depends on what else runs.
+ */
+typedef struct gm_paged_attn_args {
+  const void* q;             /* [n_seq][n_head][head_dim] in q_type */
+  const void* k_pages;
+  const void* v_pages;
+  const int32_t* block_table;
+  const int32_t* lengths;    /* [n_seq] */
+  const void* gate;          /* [n_seq][n_head][head_dim] in gate_type, or NULL */
+  void* out;                 /* [n_seq][n_head][head_dim] in q_type, contiguous, 16-byte aligned */
+  int64_t q_stride_t, q_stride_h, gate_stride_t, gate_stride_h;
+  int64_t table_stride;      /* elements between the tables of two sequences */
+  float scale;
+  int32_t n_seq, n_head, n_head_kv, head_dim;
+  int32_t n_pages, page_size, table_width;
+  int32_t q_type, cache_type, gate_type;
+} gm_paged_attn_args;
+/* Workspace bytes of gm_paged_attention (0 on bad arguments; reads no pointer). */
+size_t gm_paged_attention_workspace_bytes(const gm_paged_attn_args* a);
+int gm_paged_attention(const gm_paged_attn_args* a, void* ws, size_t ws_bytes, void* stream);
+
+/*
+ * Causal attention over packed prompts: sequence b has the query rows cu_q[b] ..
+ * cu_q[b + 1] - 1 of q, gate and out, and n_k keys; its row i sees keys 0 ..
+ * n_k - n_q + i (so a prompt may follow keys that are there already), and gives
+ * zeros if that is none.  Keys and values are packed rows cu_k[b] .. cu_k[b + 1]
+ * - 1 of k / v (block_table NULL; rows 16-byte aligned), or the first lengths[b]
+ * positions of a cache.
+ * Rows of out before cu_q[0] and from cu_q[n_seq] on are left as they were.
+ * q, k, v and out share one type, F16 or BF16; scores and sums are fp32, the
+ * probabilities are rounded to that type for their product with v.
+ * n_seq is at most 8192; offsets outside the arrays count as their ends.
+ */
+typedef struct gm_prompt_attn_args {
+  const void* q;             /* [n_q][n_head][head_dim] */
+  const void* k;             /* packed [n_k][n_head_kv][head_dim], strides below, or the pages */
+  const void* v;
+  const int32_t* cu_q;       /* [n_seq + 1], ascending */
+  const int32_t* cu_k;       /* [n_seq + 1], ascending (packed keys) */
+  const int32_t* block_table;
+  const int32_t* lengths;    /* [n_seq] (pages) */
+  const void* gate;          /* [n_q][n_head][head_dim] in gate_type, or NULL */
+  void* out;                 /* [n_q][n_head][head_dim], contiguous, 16-byte aligned */
+  int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h;
+  int64_t v_stride_t, v_stride_h, gate_stride_t, gate_stride_h;
+  int64_t table_stride;
+  float scale;
+  int32_t n_q, n_k, n_seq, n_head, n_head_kv;
+  int32_t head_dim, n_pages, page_size, table_width;
+  int32_t type, gate_type;
+} gm_prompt_attn_args;
+int gm_prompt_attention(const gm_prompt_attn_args* a, void* stream);
+
+/*
+ * One token per row of logits [n_row][vocab]: weights w_i = exp((x_i - max x) / t)
+ * in 64 bits; of them the top_k largest (0: all), of those the shortest run from
+ * the largest on whose sum reaches top_p of theirs (at least one; >= 1: all), of
+ * those the ones with w >= min_p; and of what is left the first token, in the
+ * vocabulary's order, whose running sum passes u times the total.  Equal logits
+ * rank by index, lowest first.  t <= 0 takes the largest logit.  -inf and NaN
+ * logits are never taken; a row of nothing else gives -1.  Where the largest logit
+ * is +inf, only +inf ones count.  A parameter is a device array of one value per
+ * row, or (NULL) the value beside it.  ids: int64 [n_row].
+ * No counterpart in the reference (its CLIs take the argmax on the host).
+ */
+typedef struct gm_sample_args {
+  const void* logits;        /* rows in type, row_stride elements apart */
+  const float* u;            /* [n_row], in [0, 1) */
+  const float* temperature;  /* [n_row] or NULL */
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  int64_t* ids;
+  int64_t row_stride;
+  float temperature_all;
+  int32_t top_k_all;
+  float top_p_all, min_p_all;
+  int32_t n_row, vocab, type;
+} gm_sample_args;
+/* Workspace bytes of gm_sample (0 on bad arguments; reads no pointer). */
+size_t gm_sample_workspace_bytes(const gm_sample_args* a);
+int gm_sample(const gm_sample_args* a, void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

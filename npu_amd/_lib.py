@@ -78,6 +78,63 @@ class GmSsmLayer(ctypes.Structure):
     ]
 
 
+class GmRopeAppendArgs(ctypes.Structure):
+    """Mirror of ``gm_rope_append_args`` (include/npu_amd.h)."""
+
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("positions", _vp), ("inv_freq", _vp), ("axis", _vp),
+        ("q_norm", _vp), ("k_norm", _vp), ("q_out", _vp), ("k_pages", _vp), ("v_pages", _vp), ("slots", _vp),
+        ("q_stride_t", _i64), ("q_stride_h", _i64), ("k_stride_t", _i64), ("k_stride_h", _i64),
+        ("v_stride_t", _i64), ("v_stride_h", _i64), ("n_rows", _i64),
+        ("eps", _f32),
+        ("T", _i32), ("n_axes", _i32), ("n_head", _i32), ("n_head_kv", _i32),
+        ("head_dim", _i32), ("rope_dim", _i32), ("in_type", _i32), ("out_type", _i32), ("cache_type", _i32),
+    ]
+
+
+class GmPagedAttnArgs(ctypes.Structure):
+    """Mirror of ``gm_paged_attn_args`` (include/npu_amd.h)."""
+
+    _fields_ = [
+        ("q", _vp), ("k_pages", _vp), ("v_pages", _vp), ("block_table", _vp), ("lengths", _vp), ("gate", _vp),
+        ("out", _vp),
+        ("q_stride_t", _i64), ("q_stride_h", _i64), ("gate_stride_t", _i64), ("gate_stride_h", _i64),
+        ("table_stride", _i64),
+        ("scale", _f32),
+        ("n_seq", _i32), ("n_head", _i32), ("n_head_kv", _i32), ("head_dim", _i32),
+        ("n_pages", _i32), ("page_size", _i32), ("table_width", _i32),
+        ("q_type", _i32), ("cache_type", _i32), ("gate_type", _i32),
+    ]
+
+
+class GmPromptAttnArgs(ctypes.Structure):
+    """Mirror of ``gm_prompt_attn_args`` (include/npu_amd.h)."""
+
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("cu_q", _vp), ("cu_k", _vp), ("block_table", _vp), ("lengths", _vp),
+        ("gate", _vp), ("out", _vp),
+        ("q_stride_t", _i64), ("q_stride_h", _i64), ("k_stride_t", _i64), ("k_stride_h", _i64),
+        ("v_stride_t", _i64), ("v_stride_h", _i64), ("gate_stride_t", _i64), ("gate_stride_h", _i64),
+        ("table_stride", _i64),
+        ("scale", _f32),
+        ("n_q", _i32), ("n_k", _i32), ("n_seq", _i32), ("n_head", _i32), ("n_head_kv", _i32),
+        ("head_dim", _i32), ("n_pages", _i32), ("page_size", _i32), ("table_width", _i32),
+        ("type", _i32), ("gate_type", _i32),
+    ]
+
+
+class GmSampleArgs(ctypes.Structure):
+    """Mirror of ``gm_sample_args`` (include/npu_amd.h)."""
+
+    _fields_ = [
+        ("logits", _vp), ("u", _vp), ("temperature", _vp), ("top_k", _vp), ("top_p", _vp), ("min_p", _vp),
+        ("ids", _vp),
+        ("row_stride", _i64),
+        ("temperature_all", _f32), ("top_k_all", _i32), ("top_p_all", _f32), ("min_p_all", _f32),
+        ("n_row", _i32), ("vocab", _i32), ("type", _i32),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/npu_amd.h declares.
 SIGNATURES = {
     "gm_last_error": (ctypes.c_char_p, []),
@@ -115,6 +172,12 @@ SIGNATURES = {
     "gm_ssm_prefill": (_i32, [ctypes.POINTER(GmSsmLayer), _vp, _vp, _i32, _vp, _vp, _i32, _vp, _sz, _vp]),
     "gm_moe_forward_acc": (_i32, [ctypes.POINTER(GmMoeLayer), _vp, _vp, _i32, _vp, _sz, _vp]),
     "gm_rms_norm": (_i32, [_vp, _vp, _i32, _i32, _f32, _vp, _vp]),
+    "gm_rope_append": (_i32, [ctypes.POINTER(GmRopeAppendArgs), _vp]),
+    "gm_paged_attention_workspace_bytes": (_sz, [ctypes.POINTER(GmPagedAttnArgs)]),
+    "gm_paged_attention": (_i32, [ctypes.POINTER(GmPagedAttnArgs), _vp, _sz, _vp]),
+    "gm_prompt_attention": (_i32, [ctypes.POINTER(GmPromptAttnArgs), _vp]),
+    "gm_sample_workspace_bytes": (_sz, [ctypes.POINTER(GmSampleArgs)]),
+    "gm_sample": (_i32, [ctypes.POINTER(GmSampleArgs), _vp, _sz, _vp]),
 }
 
 _LIB: ctypes.CDLL | None = None

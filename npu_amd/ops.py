@@ -188,3 +188,279 @@ def moe_chain_fused(layers, T: int) -> bool:
     """Whether gm_moe_chain links consecutive layers at ``T`` tokens (mode 1 or 2 above)
     rather than running one gm_moe_forward per layer."""
     return moe_chain_mode(layers, T) > 0
+
+
+# ------------------------------------------------------------ serving a batch
+_ELEM = {torch.float32: L.GM_QTYPE_F32, torch.float16: L.GM_QTYPE_F16, torch.bfloat16: L.GM_QTYPE_BF16}
+
+
+def _elem(t: torch.Tensor, name: str, among=_ELEM) -> int:
+    if t.dtype not in among:
+        raise TypeError(f"{name} must be {' or '.join(str(d) for d in among)}, got {t.dtype}")
+    return _ELEM[t.dtype]
+
+
+def _rows(t: torch.Tensor, name: str, shape) -> torch.Tensor:
+    """t, of the given shape ([.., heads, head_dim]) and with contiguous rows of head_dim."""
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    if t.stride(-1) != 1:
+        raise ValueError(f"{name}: the last dim must be contiguous")
+    return t
+
+
+def _ints(t: torch.Tensor, name: str, shape) -> torch.Tensor:
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name} must be int32, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    return t
+
+
+_T16 = (torch.bfloat16, torch.float16)
+
+
+def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor):
+    """(type, n_pages, page_size, n_head_kv, head_dim) of a cache."""
+    ct = _elem(k_pages, "k_pages", _T16)
+    if k_pages.dim() != 4:
+        raise ValueError(f"k_pages must be [n_pages, page_size, n_head_kv, head_dim], got {list(k_pages.shape)}")
+    if v_pages.dtype != k_pages.dtype or v_pages.shape != k_pages.shape:
+        raise ValueError("v_pages must have k_pages' shape and type")
+    if not (k_pages.is_contiguous() and v_pages.is_contiguous()):
+        raise ValueError("k_pages and v_pages must be contiguous")
+    return (ct, *k_pages.shape)
+
+
+def _out(out: torch.Tensor | None, shape, dtype: torch.dtype, like: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    if out.shape != shape or out.dtype != dtype or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous {list(shape)} {dtype}, got {list(out.shape)} {out.dtype}")
+    return out
+
+
+def _one_device(first: torch.Tensor, *others: torch.Tensor | None) -> torch.device:
+    dev = first.device
+    if dev.type != "cuda":
+        raise ValueError("tensors must be on the GPU")
+    for t in others:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
+    return dev
+
+
+def _ptr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def _enqueue(dev: torch.device, name: str, args, ws_bytes=None) -> None:
+    """Call the entry point ``name`` on ``dev``'s current stream; with ``ws_bytes`` (the name of
+    its size query) it gets a workspace of its own."""
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _enqueue(dev, name, args, ws_bytes)
+    lib = L.lib()
+    ref = ctypes.byref(args)
+    if ws_bytes is None:
+        rc = getattr(lib, name)(ref, L.stream_ptr())
+    else:
+        n = getattr(lib, ws_bytes)(ref)
+        if n == 0:
+            L.check(L.GM_EINVAL, name)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        rc = getattr(lib, name)(ref, ws.data_ptr(), n, L.stream_ptr())
+    L.check(rc, name)
+
+
+def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
+                k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tensor, *,
+                axis: torch.Tensor | None = None, q_norm: torch.Tensor | None = None,
+                k_norm: torch.Tensor | None = None, eps: float = 1e-6, out: torch.Tensor | None = None,
+                out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """The step between the projections and the attention of many sequences' new tokens:
+    rotated (and, with ``q_norm`` / ``k_norm`` [head_dim] fp32, RMS-normed) q is returned, k
+    and v go to the cache (``gm_rope_append``).
+
+    q [T, n_head, head_dim], k and v [T, n_head_kv, head_dim] (one type; views into a
+    projection's rows are fine); positions int32 [T] or [n_axes, T]; inv_freq fp64
+    [rope_dim / 2], radians per position, and axis int32 [rope_dim / 2], the axis that turns
+    each pair (``qwen_core.build_rope_axes``); k_pages / v_pages [n_pages, page_size,
+    n_head_kv, head_dim] bf16 or fp16; slots int32 [T], the cache row of each token (page
+    times page_size plus row), negative for none, no row twice.  The result has the cache's
+    type, or ``out_dtype``.  A packed buffer [T, n_head_kv, head_dim] viewed as one page,
+    with slots 0 .. T - 1, serves where no cache is wanted."""
+    in_type = _elem(q, "q")
+    ct, n_pages, page, hkv, dh = _pages(k_pages, v_pages)
+    if q.dim() != 3:
+        raise ValueError(f"q must be [T, n_head, head_dim], got {list(q.shape)}")
+    T, hq, _ = q.shape
+    _rows(q, "q", (T, hq, dh))
+    _rows(k, "k", (T, hkv, dh))
+    _rows(v, "v", (T, hkv, dh))
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("q, k and v must have one type")
+    n_axes = positions.shape[0] if positions.dim() == 2 else 1
+    _ints(positions, "positions", (n_axes, T) if positions.dim() == 2 else (T,))
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise TypeError("inv_freq must be contiguous float64 [rope_dim / 2]")
+    half = inv_freq.shape[0]
+    _ints(slots, "slots", (T,))
+    if axis is not None:
+        _ints(axis, "axis", (half,))
+    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if w is not None and (w.dtype != torch.float32 or w.shape != (dh,) or not w.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous float32 [{dh}]")
+    if not (positions.is_contiguous() and slots.is_contiguous() and (axis is None or axis.is_contiguous())):
+        raise ValueError("positions, slots and axis must be contiguous")
+    dev = _one_device(q, k, v, positions, inv_freq, k_pages, v_pages, slots, axis, q_norm, k_norm, out)
+    out = _out(out, (T, hq, dh), out_dtype or (k_pages.dtype if out is None else out.dtype), q)
+    a = L.GmRopeAppendArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(),
+                           _ptr(axis), _ptr(q_norm), _ptr(k_norm), out.data_ptr(), k_pages.data_ptr(),
+                           v_pages.data_ptr(), slots.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1),
+                           v.stride(0), v.stride(1), n_pages * page, eps, T, n_axes, hq, hkv, dh, 2 * half, in_type,
+                           _elem(out, "out"), ct)
+    _enqueue(dev, "gm_rope_append", a)
+    return out
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                    lengths: torch.Tensor, *, scale: float | None = None, gate: torch.Tensor | None = None,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one new token per sequence over a paged cache (``gm_paged_attention``):
+    q [n_seq, n_head, head_dim] in fp32 or the cache's type, block_table int32 [n_seq, width]
+    (page numbers in order; entries past a sequence's last page are not read), lengths int32
+    [n_seq] with the new token counted.  ``scale`` (positive) defaults to head_dim ** -0.5; ``gate`` of
+    q's shape multiplies the result by its sigmoid.  Sequences of length 0 give zeros.
+    Lengths and tables are read on the device only, so the call may be captured and replayed
+    with other ones."""
+    qt = _elem(q, "q")
+    ct, n_pages, page, hkv, dh = _pages(k_pages, v_pages)
+    if q.dim() != 3:
+        raise ValueError(f"q must be [n_seq, n_head, head_dim], got {list(q.shape)}")
+    B, hq, _ = q.shape
+    _rows(q, "q", (B, hq, dh))
+    _ints(lengths, "lengths", (B,))
+    if block_table.dim() != 2:
+        raise ValueError(f"block_table must be [n_seq, width], got {list(block_table.shape)}")
+    width = block_table.shape[1]
+    _ints(block_table, "block_table", (B, width))
+    if (width > 1 and block_table.stride(1) != 1) or not lengths.is_contiguous():
+        raise ValueError("lengths and the rows of block_table must be contiguous")
+    gt = gs0 = gs1 = 0
+    if gate is not None:
+        gt = _elem(gate, "gate")
+        _rows(gate, "gate", (B, hq, dh))
+        gs0, gs1 = gate.stride(0), gate.stride(1)
+    dev = _one_device(q, k_pages, v_pages, block_table, lengths, gate, out)
+    out = _out(out, (B, hq, dh), q.dtype, q)
+    if B == 0:
+        return out
+    a = L.GmPagedAttnArgs(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(),
+                          lengths.data_ptr(), _ptr(gate), out.data_ptr(), q.stride(0), q.stride(1), gs0, gs1,
+                          block_table.stride(0) if B > 1 else width, dh ** -0.5 if scale is None else scale, B, hq,
+                          hkv, dh, n_pages, page, width, qt, ct, gt)
+    _enqueue(dev, "gm_paged_attention", a, "gm_paged_attention_workspace_bytes")
+    return out
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, *,
+                     cu_k: torch.Tensor | None = None, block_table: torch.Tensor | None = None,
+                     lengths: torch.Tensor | None = None, scale: float | None = None,
+                     gate: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention over packed prompts (``gm_prompt_attention``): q [n_q, n_head,
+    head_dim] bf16 or fp16, sequence b in rows cu_q[b] .. cu_q[b + 1] - 1 (int32 [n_seq + 1]).
+    Keys and values are k, v [n_k, n_head_kv, head_dim] packed by cu_k (cu_q where it is
+    None), or, with block_table [n_seq, width] and lengths [n_seq] (both int32), the first
+    lengths[b] positions of cache pages k, v [n_pages, page_size, n_head_kv, head_dim].  A
+    sequence's last query row sees all its keys, so a prompt may follow cached ones.  Rows
+    that see no key give zeros; rows of ``out`` outside the sequences are left as they were."""
+    paged = block_table is not None
+    if paged != (lengths is not None) or (paged and cu_k is not None):
+        raise ValueError("keys are packed (cu_k) or in pages (block_table and lengths)")
+    qt = _elem(q, "q", _T16)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("q, k and v must have one type")
+    if q.dim() != 3 or k.dim() != (4 if paged else 3):
+        raise ValueError("q must be [n_q, n_head, head_dim], k and v [n_k, n_head_kv, head_dim] or pages")
+    n_q, hq, dh = q.shape
+    n_seq = cu_q.shape[0] - 1
+    if cu_q.dim() != 1 or n_seq < 0:
+        raise ValueError("cu_q must be [n_seq + 1]")
+    _ints(cu_q, "cu_q", (n_seq + 1,))
+    _rows(q, "q", (n_q, hq, dh))
+    n_k = n_pages = page = width = ts = 0
+    if paged:
+        _, n_pages, page, hkv, _ = _pages(k, v)
+        if block_table.dim() != 2 or block_table.shape[0] != n_seq:
+            raise ValueError(f"block_table must be [{n_seq}, width], got {list(block_table.shape)}")
+        width = block_table.shape[1]
+        _ints(block_table, "block_table", (n_seq, width))
+        _ints(lengths, "lengths", (n_seq,))
+        if (width > 1 and block_table.stride(1) != 1) or not lengths.is_contiguous():
+            raise ValueError("lengths and the rows of block_table must be contiguous")
+        ts = block_table.stride(0) if n_seq > 1 else width
+        ks0 = ks1 = vs0 = vs1 = 0
+    else:
+        n_k, hkv, _ = k.shape
+        cu_k = cu_q if cu_k is None else _ints(cu_k, "cu_k", (n_seq + 1,))
+        ks0, ks1, vs0, vs1 = k.stride(0), k.stride(1), v.stride(0), v.stride(1)
+    if k.shape[-1] != dh:
+        raise ValueError(f"k has head_dim {k.shape[-1]}, q {dh}")
+    _rows(k, "k", k.shape)
+    _rows(v, "v", k.shape)
+    if not cu_q.is_contiguous() or (cu_k is not None and not cu_k.is_contiguous()):
+        raise ValueError("cu_q and cu_k must be contiguous")
+    gt = gs0 = gs1 = 0
+    if gate is not None:
+        gt = _elem(gate, "gate")
+        _rows(gate, "gate", (n_q, hq, dh))
+        gs0, gs1 = gate.stride(0), gate.stride(1)
+    dev = _one_device(q, k, v, cu_q, cu_k, block_table, lengths, gate, out)
+    out = _out(out, (n_q, hq, dh), q.dtype, q)
+    a = L.GmPromptAttnArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), _ptr(cu_k), _ptr(block_table),
+                           _ptr(lengths), _ptr(gate), out.data_ptr(), q.stride(0), q.stride(1), ks0, ks1, vs0, vs1,
+                           gs0, gs1, ts, dh ** -0.5 if scale is None else scale, n_q, n_k, n_seq, hq, hkv, dh,
+                           n_pages, page, width, qt, gt)
+    _enqueue(dev, "gm_prompt_attention", a)
+    return out
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: float | torch.Tensor = 1.0,
+           top_k: int | torch.Tensor | None = None, top_p: float | torch.Tensor | None = None,
+           min_p: float | torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """One token per row of logits [n_row, vocab] (fp32, bf16 or fp16; rows may be strided)
+    at the given uniform numbers u fp32 [n_row] in [0, 1): int64 [n_row] (``gm_sample``).
+
+    Filters in this order: the top_k largest (0: all), the shortest run of the largest whose
+    weight reaches top_p of theirs, the ones of at least min_p times the largest weight; the
+    pick is the inverse of the running sum of what is left, in the vocabulary's order.  Each
+    parameter is one value or a tensor of one per row (fp32; top_k int32).  temperature 0 is
+    the argmax, lowest index first.  A row without a logit above -inf gives -1."""
+    lt = _elem(logits, "logits")
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError(f"logits must be [n_row, vocab], got {list(logits.shape)}")
+    B, V = logits.shape
+    if V > 1 and logits.stride(1) != 1:
+        raise ValueError("logits: the last dim must be contiguous")
+    if u.dtype != torch.float32 or u.shape != (B,) or not u.is_contiguous():
+        raise ValueError(f"u must be contiguous float32 [{B}]")
+    held, alone = [], []
+    for name, val, dt, none in (("temperature", temperature, torch.float32, 1.0), ("top_k", top_k, torch.int32, 0),
+                                ("top_p", top_p, torch.float32, 1.0), ("min_p", min_p, torch.float32, 0.0)):
+        if isinstance(val, torch.Tensor):
+            if val.dtype != dt or val.shape != (B,) or not val.is_contiguous():
+                raise ValueError(f"{name} must be contiguous {dt} [{B}] or one value")
+            held.append(val)
+            alone.append(none)
+        else:
+            held.append(None)
+            alone.append(none if val is None else val)
+    dev = _one_device(logits, u, *held, out)
+    out = _out(out, (B,), torch.int64, logits)
+    if B == 0:
+        return out
+    a = L.GmSampleArgs(logits.data_ptr(), u.data_ptr(), *(_ptr(t) for t in held), out.data_ptr(),
+                       logits.stride(0) if B > 1 else V, *alone, B, V, lt)
+    _enqueue(dev, "gm_sample", a, "gm_sample_workspace_bytes")
+    return out
