@@ -4,18 +4,19 @@
 // The pick is that of the definition in 64 bits: weights w = e^((x - max) / t) and
 // all their sums are fp64, so that u times the total falls between the same two
 // running sums.  fp64 FMAs run at the fp32 rate here; the exponential is a table of
-// 64 powers in LDS and five terms (14 instructions instead of the library's 40).
+// 64 powers in LDS and five terms.
 //
-// k_sample_groups   every group of 512 logits: its maximum and, for rows without a
-//                   top-k, its sum of weights.  The one pass over all logits.
-// k_sample_pick     one block per row.  Whatever passes the filters is at least the
-//                   k-th largest group maximum (k groups hold such a value each) or
-//                   what min-p leaves, so few groups are read again; up to kCand
-//                   candidates are ranked against each other in LDS.  More than that
-//                   (a nucleus without top-k, a large k): a histogram of the distance
-//                   from the maximum finds the bin where the filter ends, and only
-//                   that bin's values are ranked (or cut bit by bit, if they too are
-//                   many).
+// k_sample_groups   every group of 512 logits: its maximum, the maximum of every lane's
+//                   8 and, for rows without a top-k, the group's sum of weights.  The
+//                   one pass over all logits.
+// k_sample_pick     one block per row.  A histogram of the lanes' maxima over their
+//                   distance from the row's finds a distance that the filters cannot
+//                   pass: where k maxima are nearer, or maxima that weigh top_p of the
+//                   total, or by min-p itself.  Only lanes with a maximum that near are
+//                   read again, and up to kCand candidates are ranked against each
+//                   other in LDS.  More than that (a flat nucleus, a large k): the same
+//                   histogram over all values finds the bin where the filter ends, and
+//                   only that bin's are ranked (or cut bit by bit, if they too are many).
 // Kept tokens run in the vocabulary's order, so nothing is ever sorted as a whole.
 // No result depends on the order of atomics: they count, or add fixed-point values.
 // Bound: HBM and, without top-k, the fp64 exponentials of the first kernel; for few
@@ -29,6 +30,7 @@ constexpr int kGroup = 512;         // logits of a group: 8 per lane of a wave
 constexpr int kCand = 1024;         // candidates ranked in LDS, one per thread
 constexpr int kBins = 2048;         // bins of the distance from the maximum ...
 constexpr float kBinsPerE = 32.f;   // ... 1/32 wide, in units of the temperature
+constexpr int kList = 4096;         // lanes of 8 logits that are read again
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kPosInf = __builtin_inff();
 
@@ -38,6 +40,7 @@ struct Smp {
   gm_sample_args a;
   float* gmax;       // [n_row][ng]
   double* gsum;      // [n_row][ng]
+  void* lmax;        // [n_row][ng][64] in the logits' type
   int ng;
   bool vec;          // rows start at multiples of 16 bytes
 };
@@ -71,28 +74,32 @@ __device__ __forceinline__ void exp_table(double* tab) {
   if (threadIdx.x < 64) tab[threadIdx.x] = exp2((double)threadIdx.x * (1.0 / 64));
 }
 
-// e^y for y <= 0 within 2e-16: y = k ln2 / 64 + z, |z| < 0.0055, the powers of
-// 2^(1/64) from the table.
+constexpr double kUnits = 92.332482616893656877;       // 64 / ln 2
+constexpr double kFar = -700.0 * kUnits;               // weights below e^-700 count as 0
+
+// 2^(y / 64), kFar <= y <= 0, within 3e-16 of it and 2e-16 |y / 64| more: y = k + f with
+// |f| <= 1/2, 2^(k % 64 / 64) from the table, 2^(k / 64) straight into the exponent.  k
+// is in the low bits of a sum with 1.5 x 2^52.
 __device__ __forceinline__ double fexp(double y, const double* tab) {
-  y = fmax(y, -800.0);                                 // 0 below -745
-  const double k = rint(y * 92.332482616893656877);    // 64 / ln 2
-  double z = fma(k, -0x1.62e42fefa39efp-7, y);         // ln 2 / 64, its leading bits and the rest
-  z = fma(k, -0x1.abc9e3b39803fp-62, z);
-  double p = fma(z, 1.0 / 120, 1.0 / 24);
-  p = fma(z, p, 1.0 / 6);
-  p = fma(z, p, 0.5);
-  p = fma(z, p, 1.0);
-  const int ki = (int)k;
+  constexpr double magic = 6755399441055744.0, c = 0.010830424696249145;      // ln 2 / 64
+  const double t = y + magic;
+  const int ki = (int)(uint32_t)__double_as_longlong(t);
+  const double f = y - (t - magic);
+  double p = fma(f, c * c * c * c * c / 120, c * c * c * c / 24);
+  p = fma(f, p, c * c * c / 6);
+  p = fma(f, p, c * c / 2);
+  p = fma(f, p, c);
   const double s = tab[ki & 63];
-  return ldexp(fma(s, z * p, s), ki >> 6);
+  return __longlong_as_double(__double_as_longlong(fma(s, f * p, s)) + ((long long)(ki >> 6) << 52));
 }
 
-// The weight of x beside the maximum m (inv = 1 / t).
-__device__ __forceinline__ double weight(float x, float m, double inv, const double* tab) {
+// The weight of x beside the maximum m; units = 64 / (ln 2 t).
+__device__ __forceinline__ double weight(float x, float m, double units, const double* tab) {
   if (!(x > kNegInf)) return 0.0;                      // NaN, -inf
   if (x == m) return 1.0;
   if (m == kPosInf) return 0.0;
-  return fexp(((double)x - (double)m) * inv, tab);
+  const double y = ((double)x - (double)m) * units;
+  return y < kFar ? 0.0 : fexp(y, tab);
 }
 
 // The 8 logits of a lane in group gr; index of the j-th: at(j).  Past the end -inf.
@@ -101,9 +108,9 @@ struct Lane8 {
   int i0, step;
   __device__ __forceinline__ int at(int j) const { return i0 + (j & 3) + (j >> 2) * step; }
 };
-__device__ __forceinline__ Lane8 load8(const Smp& P, int row, int gr) {
+__device__ __forceinline__ Lane8 load8(const Smp& P, int row, int gr, int lane) {
   const gm_sample_args& A = P.a;
-  const int lane = threadIdx.x & 63, V = A.vocab;
+  const int V = A.vocab;
   Lane8 r;
   // fp32: two loads of four, 256 apart; 16 bits: one of eight
   const bool f32 = A.type == GM_QTYPE_F32;
@@ -135,6 +142,22 @@ __device__ __forceinline__ Lane8 load8(const Smp& P, int row, int gr) {
   return r;
 }
 
+__device__ __forceinline__ Lane8 load8(const Smp& P, int row, int gr) { return load8(P, row, gr, threadIdx.x & 63); }
+
+// Maximum over the wave's lanes.
+__device__ __forceinline__ float wave_max64(float v) {
+  v = fmaxf(v, GM_DPP_F(v, GM_ROW_ROR8));
+  v = fmaxf(v, GM_DPP_F(v, GM_ROW_ROR4));
+  v = fmaxf(v, GM_DPP_F(v, GM_QPERM_2301));
+  v = fmaxf(v, GM_DPP_F(v, GM_QPERM_1032));
+  const int b = __builtin_bit_cast(int, v);
+  const float r0 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 0));
+  const float r1 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 16));
+  const float r2 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 32));
+  const float r3 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 48));
+  return fmaxf(fmaxf(r0, r1), fmaxf(r2, r3));
+}
+
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
@@ -146,6 +169,9 @@ __device__ __forceinline__ double wave_sum(double v) {
   return v;
 }
 
+// U groups of a wave, loaded together: 4, or 1 where there are few rows (one row of
+// 248,320: 4.5 us with 4).
+template <int U>
 __global__ void __launch_bounds__(256) k_sample_groups(Smp P) {
   __shared__ double tab[64];
   exp_table(tab);
@@ -153,31 +179,67 @@ __global__ void __launch_bounds__(256) k_sample_groups(Smp P) {
   const int row = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const RowParam rp = row_param(P.a, row);
   const bool sums = !rp.greedy && rp.top_k == 0;
-  const double inv = 1.0 / (double)rp.t;
-  constexpr int U = 4;                                 // groups of a wave, loaded together
+  const bool lanes = !rp.greedy && (rp.top_k > 1 || rp.top_p < 1.f || rp.min_p > 0.f);
+  const double units = kUnits / (double)rp.t;
   const int g0 = (blockIdx.x * 4 + wave) * U;
   Lane8 v[U];
 #pragma unroll
   for (int u = 0; u < U; ++u)
     if (g0 + u < P.ng) v[u] = load8(P, row, g0 + u);
+  double s[U];
+  float gm[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    if (g0 + u >= P.ng) break;
+    s[u] = 0.0;
+    gm[u] = kNegInf;
+    if (g0 + u >= P.ng) continue;
     float m = v[u].x[0];
 #pragma unroll
     for (int j = 1; j < 8; ++j) m = fmaxf(m, v[u].x[j]);
-    m = wave_max(m);
-    double s = 0.0;
-    if (sums && m > kNegInf) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s += weight(v[u].x[j], m, inv, tab);
-      s = wave_sum(s);
+    if (lanes) {
+      const int64_t at = ((int64_t)row * P.ng + g0 + u) * 64 + lane;
+      if (P.a.type == GM_QTYPE_F32) static_cast<float*>(P.lmax)[at] = m;
+      else if (P.a.type == GM_QTYPE_BF16) static_cast<uint16_t*>(P.lmax)[at] = (uint16_t)GmT16<GM_QTYPE_BF16>::pack(m, m);
+      else static_cast<uint16_t*>(P.lmax)[at] = (uint16_t)GmT16<GM_QTYPE_F16>::pack(m, m);
     }
-    if (lane == 0) {
-      P.gmax[(int64_t)row * P.ng + g0 + u] = m;
-      P.gsum[(int64_t)row * P.ng + g0 + u] = s;
+    gm[u] = m = wave_max64(m);
+    if (sums && m > kNegInf) {
+      float low = v[u].x[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) low = fminf(low, v[u].x[j]);
+      if (m < kPosInf && !__any(!(((double)low - (double)m) * units >= kFar))) {
+        // the usual group: all finite and near enough (77 us with the tests per value at
+        // 256 rows of 248,320)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[u] += fexp(((double)v[u].x[j] - (double)m) * units, tab);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[u] += weight(v[u].x[j], m, units, tab);
+      }
     }
   }
+  if (sums) {
+    if constexpr (U == 4) {
+      // four sums over the lanes in 7 exchanges: pairs of lanes first take two groups
+      // each, then one; lane l ends with group l % 4
+      const bool o1 = lane & 1, o2 = lane & 2;
+      const double a = (o1 ? s[1] : s[0]) + __shfl_xor(o1 ? s[0] : s[1], 1, 64);
+      const double b = (o1 ? s[3] : s[2]) + __shfl_xor(o1 ? s[2] : s[3], 1, 64);
+      double c = (o2 ? b : a) + __shfl_xor(o2 ? a : b, 2, 64);
+#pragma unroll
+      for (int o = 4; o < 64; o <<= 1) c += __shfl_xor(c, o, 64);
+      if (lane < 4 && g0 + lane < P.ng) P.gsum[(int64_t)row * P.ng + g0 + lane] = c;
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const double c = wave_sum(s[u]);
+        if (lane == 0 && g0 + u < P.ng) P.gsum[(int64_t)row * P.ng + g0 + u] = c;
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (lane == u && g0 + u < P.ng) P.gmax[(int64_t)row * P.ng + g0 + u] = gm[u];
 }
 
 // ---- block-wide steps of k_sample_pick (1024 threads)
@@ -204,6 +266,10 @@ __device__ __forceinline__ int block_min(int v, int* red) {
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) m = min(m, red[w]);
   return m;
+}
+
+__device__ __forceinline__ int block_max_u(uint32_t v, int* red) {
+  return (int)~(uint32_t)(block_min((int)(~v ^ 0x80000000u), red) ^ 0x80000000u);
 }
 
 // Running sum over the threads, the own value with it; all: the sum.
@@ -251,6 +317,8 @@ struct Shared {
   unsigned int cnt[kBins];
 };
 
+static_assert(sizeof(Shared::mass) >= kList * sizeof(int));
+
 // Where the filters end: kept are the values above `key`, and of that value the
 // indices up to `id`.
 struct Cut {
@@ -265,7 +333,8 @@ __device__ __forceinline__ bool kept(float x, int i, const Cut& c) {
 struct Row {
   int row;
   float xmax;
-  double inv;
+  float per_bin;     // bins per unit of x
+  double units;
   double fix;        // fixed point of the histogram's masses: the sum of all fits 63 bits
 };
 
@@ -361,52 +430,100 @@ __device__ __forceinline__ void hist_find(Shared& S, bool by_count, unsigned lon
   __syncthreads();
 }
 
+// The bin of a value by its distance from the maximum; it never falls as x does.
 __device__ __forceinline__ int dist_bin(float x, const Row& R) {
   if (!(x > kNegInf)) return -1;
   if (x == R.xmax) return 0;
-  if (R.xmax == kPosInf) return kBins - 1;
-  const double d = ((double)R.xmax - (double)x) * R.inv * (double)kBinsPerE;
-  return d < (double)(kBins - 1) ? (int)d : kBins - 1;
+  const float d = (R.xmax - x) * R.per_bin;
+  return d < (float)(kBins - 1) ? (int)d : kBins - 1;
+}
+
+// For the groups of this wave that may hold something of bin `limit` or nearer, four
+// at a time: f(group, its values).
+template <typename F>
+__device__ __forceinline__ void each_group(const Smp& P, const float* gmax, const Row& R, int limit, F f) {
+  constexpr int U = 4;
+  for (int g0 = (threadIdx.x >> 6) * U; g0 < P.ng; g0 += kWaves * U) {
+    Lane8 v[U];
+    bool on[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int b = g0 + u < P.ng ? dist_bin(gmax[g0 + u], R) : -1;
+      on[u] = b >= 0 && b <= limit;
+      if (on[u]) v[u] = load8(P, R.row, g0 + u);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (on[u]) f(g0 + u, v[u]);
+  }
 }
 
 // The cut at the k-th value (by_count) or where the running weight, from the
-// largest on, reaches m; *total: the weight of what is kept.
-__device__ Cut find_cut(const Smp& P, Shared& S, const float* gmax, const Row& R, bool by_count, int k, double m,
-                        double* total) {
-  const int wave = threadIdx.x >> 6;
+// largest on, reaches m; *total: the weight of what is kept.  gs[g]: group g's kept
+// weight of at least minw; *whole: whether that is all of it, or what the bin of the
+// cut keeps is not in it yet.
+__device__ Cut find_cut(const Smp& P, Shared& S, const float* gmax, double* gs, int* ec, const Row& R, int limit,
+                        bool by_count, int k, double m, double minw, double* total, bool* whole) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   hist_clear(S);
-  for (int gr = wave; gr < P.ng; gr += kWaves) {
-    const Lane8 v = load8(P, R.row, gr);
+  each_group(P, gmax, R, limit, [&](int, const Lane8& v) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int bin = dist_bin(v.x[j], R);
-      hist_add(S, bin, bin < 0 ? 0 : (unsigned long long)(weight(v.x[j], R.xmax, R.inv, S.tab) * R.fix));
+      int bin = dist_bin(v.x[j], R);
+      if (bin > limit) bin = -1;
+      unsigned long long w = 0;
+      if (bin >= 0 && !by_count) w = (unsigned long long)(weight(v.x[j], R.xmax, R.units, S.tab) * R.fix);
+      hist_add(S, bin, w);
     }
-  }
+  });
   hist_find(S, by_count, (unsigned long long)k, m, R.fix);
-  const int bin = S.bin, members = (int)S.cnt[bin];
-  int above_n = S.above_n;
-  // the weight above the bin in 64 bits, and the bin's members if they are few
+  const int bin = S.bin, members = (int)S.cnt[bin], above_n = S.above_n;
+  // the groups' weight above the bin in 64 bits, and the bin's members: how many a group
+  // has, their least and largest key, and themselves if they are few
   if (threadIdx.x == 0) S.count = 0;
+  for (int g = threadIdx.x; g < P.ng; g += kThreads) {
+    gs[g] = 0.0;
+    ec[g] = 0;
+  }
   __syncthreads();
   double sum = 0.0;
-  for (int gr = wave; gr < P.ng; gr += kWaves) {
-    const Lane8 v = load8(P, R.row, gr);
+  uint32_t least = 0xffffffffu, most = 0u;
+  each_group(P, gmax, R, bin, [&](int g, const Lane8& v) {
+    double own = 0.0;
+    int e = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int b = dist_bin(v.x[j], R);
-      if (b >= 0 && b < bin) sum += weight(v.x[j], R.xmax, R.inv, S.tab);
-      if (b == bin && members <= kCand)
-        S.cand[atomicAdd(&S.count, 1)] = (unsigned long long)~key_of(v.x[j]) << 32 | (uint32_t)v.at(j);
+      if (b >= 0 && b < bin) {
+        const double w = weight(v.x[j], R.xmax, R.units, S.tab);
+        sum += w;
+        own += w >= minw ? w : 0.0;
+      }
+      if (b == bin) {
+        const uint32_t key = key_of(v.x[j]);
+        least = min(least, key);
+        most = max(most, key);
+        ++e;
+        if (members <= kCand) S.cand[atomicAdd(&S.count, 1)] = (unsigned long long)~key << 32 | (uint32_t)v.at(j);
+      }
     }
-  }
+    own = wave_sum(own);
+    e = gm_wave_sum(e);
+    if (lane == 0) {
+      gs[g] = own;
+      ec[g] = e;
+    }
+  });
   double above;
   block_scan<double>(sum, S.dred, &above);
+  least = ~(uint32_t)block_max_u(~least, S.ired);
+  most = (uint32_t)block_max_u(most, S.ired);
   Cut c;
-  if (members <= kCand) {
+  *whole = false;
+  if (least != most && members <= kCand) {
     __syncthreads();
     const unsigned long long mine = (int)threadIdx.x < members ? S.cand[threadIdx.x] : 0;
-    const double w = (int)threadIdx.x < members ? weight(value_of(mine), R.xmax, R.inv, S.tab) : 0.0;
+    const double w = (int)threadIdx.x < members ? weight(value_of(mine), R.xmax, R.units, S.tab) : 0.0;
     const int rank = rank_candidates(S, members, mine, w);
     double all;
     const double ws = (int)threadIdx.x < members ? S.w[threadIdx.x] : 0.0;
@@ -425,96 +542,124 @@ __device__ Cut find_cut(const Smp& P, Shared& S, const float* gmax, const Row& R
     __syncthreads();
     return c;
   }
-  // many members: 11, 11 and 10 bits of the key, then the index among equals
-  uint32_t prefix = 0;
-  int shift = 21, bits = 11;
-  uint32_t known = 0;                                   // mask of the bits that are settled
+  // many members, or equals: the keys' distance from the largest in digits of 11 bits
+  // (none if all are one value; 16-bit logits leave the low bits of a key alone)
+  const int low = P.a.type == GM_QTYPE_F32 ? 0 : P.a.type == GM_QTYPE_BF16 ? 16 : 13;
+  const uint32_t span = (most - least) >> low;
   double over = above;                                  // weight above what is left
-  int over_n = above_n;
-  for (int pass = 0; pass < 3; ++pass) {
+  int over_n = above_n, equal = members;
+  uint32_t gap = 0, known = 0;                          // settled digits of the gap, and their mask
+  for (int top = 32 - __clz(span | 1) - (span == 0); top > 0;) {
+    const int bits = top < 11 ? top : 11, shift = top - bits;
     hist_clear(S);
-    for (int gr = wave; gr < P.ng; gr += kWaves) {
-      const Lane8 v = load8(P, R.row, gr);
+    each_group(P, gmax, R, bin, [&](int, const Lane8& v) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint32_t key = key_of(v.x[j]);
-        const bool on = dist_bin(v.x[j], R) == bin && (key & known) == prefix;
-        const int digit = (int)(~key >> shift & ((1u << bits) - 1));     // 0: the largest
-        hist_add(S, on ? digit : -1,
-                 on ? (unsigned long long)(weight(v.x[j], R.xmax, R.inv, S.tab) * R.fix) : 0);
+        const uint32_t d = (most - key_of(v.x[j])) >> low;
+        const bool on = dist_bin(v.x[j], R) == bin && (d & known) == gap;
+        unsigned long long w = 0;
+        if (on && !by_count) w = (unsigned long long)(weight(v.x[j], R.xmax, R.units, S.tab) * R.fix);
+        hist_add(S, on ? (int)(d >> shift & ((1u << bits) - 1)) : -1, w);
       }
-    }
+    });
     hist_find(S, by_count, by_count ? (unsigned long long)(k - over_n) : 0, m - over, R.fix);
-    const uint32_t digit = (uint32_t)S.bin;
-    over += (double)S.above / R.fix;
     over_n += S.above_n;
-    prefix |= (~digit & ((1u << bits) - 1)) << shift;
+    equal = (int)S.cnt[S.bin];
+    gap |= (uint32_t)S.bin << shift;
     known |= ((1u << bits) - 1) << shift;
-    if (pass < 2) {
-      bits = pass == 0 ? 11 : 10;
-      shift -= bits;
+    top = shift;
+    // the weight above in 64 bits: values of the settled digits nearer than this one
+    double part = 0.0;
+    const uint32_t g1 = gap, kn = known, sh = (uint32_t)shift;
+    if (by_count) {
+      // only wanted at the end, where it is formed from the cut itself
+    } else {
+      each_group(P, gmax, R, bin, [&](int, const Lane8& v) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t d = (most - key_of(v.x[j])) >> low;
+          const uint32_t before = kn & ~(((1u << bits) - 1) << sh);
+          if (dist_bin(v.x[j], R) == bin && (d & before) == (g1 & before) && (d & kn) < g1)
+            part += weight(v.x[j], R.xmax, R.units, S.tab);
+        }
+      });
     }
+    double more;
+    block_scan<double>(part, S.dred, &more);
+    over += more;
     __syncthreads();
   }
-  const int equal = (int)S.cnt[S.bin];
-  const float x = __uint_as_float(prefix & 0x80000000u ? prefix & 0x7fffffffu : ~prefix);
-  const double w1 = weight(x, R.xmax, R.inv, S.tab);
+  c.key = most - (gap << low);
+  if (by_count && span) {
+    // the weight of the bin's values above the cut's
+    double part = 0.0, more;
+    each_group(P, gmax, R, bin, [&](int, const Lane8& v) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (dist_bin(v.x[j], R) == bin && key_of(v.x[j]) > c.key) part += weight(v.x[j], R.xmax, R.units, S.tab);
+    });
+    block_scan<double>(part, S.dred, &more);
+    over += more;
+  }
+  const float x = value_of((unsigned long long)~c.key << 32);
+  const double w1 = weight(x, R.xmax, R.units, S.tab);
   double need = by_count ? (double)(k - over_n) : w1 > 0.0 ? ceil((m - over) / w1) : (double)equal;
   need = fmin(fmax(need, 1.0), (double)equal);
   const int nth = (int)need;
   *total = over + need * w1;
-  // the nth index that holds x: groups in order, 1024 at a time
-  c.key = prefix;
-  c.id = -1;
-  int seen = 0;
-  for (int g0 = 0; g0 < P.ng && c.id < 0; g0 += kThreads) {
+  if (span) {
+    // how many of exactly this value every group has
     __syncthreads();
-    for (int gr = g0 + wave; gr < min(g0 + kThreads, P.ng); gr += kWaves) {
-      const Lane8 v = load8(P, R.row, gr);
+    each_group(P, gmax, R, bin, [&](int g, const Lane8& v) {
       int e = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) e += v.x[j] > kNegInf && key_of(v.x[j]) == prefix ? 1 : 0;
+      for (int j = 0; j < 8; ++j) e += v.x[j] > kNegInf && key_of(v.x[j]) == c.key ? 1 : 0;
       e = gm_wave_sum(e);
-      if ((threadIdx.x & 63) == 0) S.id[gr - g0] = e;
-    }
+      if (lane == 0) ec[g] = e;
+    });
     __syncthreads();
-    const int own = g0 + (int)threadIdx.x < P.ng ? S.id[threadIdx.x] : 0;
-    int all;
-    const int run = block_scan<int>(own, S.ired, &all) + seen;
-    if (run >= nth && run - own < nth) {
-      S.bin = g0 + (int)threadIdx.x;
-      S.above_n = nth - (run - own);
-    }
-    __syncthreads();
-    if (seen + all >= nth) {
-      if (wave == 0) {
-        const Lane8 v = load8(P, R.row, S.bin);
-        // the group's equals in index order: as many passes as the value has places
-        int left = S.above_n, at = -1;
-        uint32_t mine = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) mine |= (v.x[j] > kNegInf && key_of(v.x[j]) == prefix ? 1u : 0u) << j;
-        while (left > 0) {
-          int best = 0x7fffffff;
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (mine >> j & 1) best = min(best, v.at(j));
-          int low = best;
-#pragma unroll
-          for (int o = 32; o > 0; o >>= 1) low = min(low, __shfl_xor(low, o, 64));
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (v.at(j) == low) mine &= ~(1u << j);
-          at = low;
-          --left;
-        }
-        if (threadIdx.x == 0) S.count = at;
-      }
-      __syncthreads();
-      c.id = S.count;
-    }
-    seen += all;
   }
+  // the nth index that holds x: the groups in order, every thread some
+  const int per = (P.ng + kThreads - 1) / kThreads, g0 = min((int)threadIdx.x * per, P.ng), g1 = min(g0 + per, P.ng);
+  int own = 0, all;
+  for (int g = g0; g < g1; ++g) own += ec[g];
+  int run = block_scan<int>(own, S.ired, &all) - own;
+  for (int g = g0; g < g1; ++g) {
+    const int e = ec[g], in = min(max(nth - run, 0), e);
+    if (e > 0 && in > 0 && run + e >= nth) {             // the group of the nth
+      S.bin = g;
+      S.above_n = nth - run;
+    }
+    if (w1 >= minw) gs[g] += (double)in * w1;
+    run += e;
+  }
+  __syncthreads();
+  *whole = span == 0;
+  if (wave == 0) {
+    const Lane8 v = load8(P, R.row, S.bin);
+    // the group's equals in index order, one after the other
+    int left = S.above_n, at = -1;
+    uint32_t mine = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mine |= (v.x[j] > kNegInf && key_of(v.x[j]) == c.key ? 1u : 0u) << j;
+    while (left > 0) {
+      int best = 0x7fffffff;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (mine >> j & 1) best = min(best, v.at(j));
+      int first = best;
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) first = min(first, __shfl_xor(first, o, 64));
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (v.at(j) == first) mine &= ~(1u << j);
+      at = first;
+      --left;
+    }
+    if (threadIdx.x == 0) S.count = at;
+  }
+  __syncthreads();
+  c.id = S.count;
   __syncthreads();
   return c;
 }
@@ -524,6 +669,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(Smp P) {
   Shared& S = *reinterpret_cast<Shared*>(dyn);
   double* gs = reinterpret_cast<double*>(dyn + sizeof(Shared));          // [ng]
   float* gmax = reinterpret_cast<float*>(gs + P.ng);                     // [ng]
+  int* ec = reinterpret_cast<int*>(gmax + P.ng);                         // [ng]
   const gm_sample_args& A = P.a;
   const int row = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   exp_table(S.tab);
@@ -537,7 +683,9 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(Smp P) {
   Row R;
   R.row = row;
   R.xmax = block_max(mx, S.fred);
-  R.inv = 1.0 / (double)rp.t;
+  const double inv = 1.0 / (double)rp.t;
+  R.units = kUnits / (double)rp.t;
+  R.per_bin = (float)(inv * (double)kBinsPerE);
   R.fix = ldexp(1.0, 62 - (32 - __clz(A.vocab)));
   if (R.xmax == kNegInf) {
     if (tid == 0) A.ids[row] = -1;
@@ -561,54 +709,98 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(Smp P) {
     return;
   }
   const bool by_p = rp.top_p < 1.f, by_k = rp.top_k > 0, by_min = rp.min_p > 0.f;
-  // ---- the least value that may be kept or counted
-  float bound = kNegInf;
-  if (by_k && rp.top_k <= P.ng) {
-    int hit = -1;
-    for (int i = tid; i < P.ng; i += kThreads) {        // the k-th largest group maximum
-      int above = 0;
-      const float own = gmax[i];
-      for (int j = 0; j < P.ng; ++j) above += gmax[j] > own || (gmax[j] == own && j < i) ? 1 : 0;
-      if (above == rp.top_k - 1) hit = i;
-    }
-    hit = -block_min(-hit, S.ired);
-    bound = gmax[hit];
-  }
-  if (by_min && !(by_k && by_p)) {
-    // what is a little below stays in: the test itself is the weight's
-    const double low = (double)R.xmax + (double)rp.t * (log((double)rp.min_p) * 1.000001 - 1e-6);
-    const float lf = (float)low;
-    bound = fmaxf(bound, lf - fabsf(lf) * 1e-6f);
-  }
   const double minw = (double)rp.min_p;
   double all = 0.0;                                     // the weight of everything
   if (!by_k) {
     double s = 0.0;
     for (int g = tid; g < P.ng; g += kThreads) {
-      const double v = gmax[g] == kNegInf ? 0.0 : P.gsum[(int64_t)row * P.ng + g] * weight(gmax[g], R.xmax, R.inv, S.tab);
+      const double v = gmax[g] == kNegInf ? 0.0 : P.gsum[(int64_t)row * P.ng + g] * weight(gmax[g], R.xmax, R.units, S.tab);
       gs[g] = v;
       s += v;
     }
     block_scan<double>(s, S.dred, &all);
   }
   const double u = (double)A.u[row];
-  // ---- few candidates: ranked in LDS
-  if (bound > kNegInf) {
-    for (int g = wave; g < P.ng; g += kWaves) {
-      if (!(gmax[g] >= bound)) continue;
-      const Lane8 v = load8(P, row, g);
+  // ---- the farthest bin that may hold something kept, or counted by a filter before
+  int limit = kBins - 1;
+  const int nl = P.ng * 64;
+  const int64_t l0 = (int64_t)row * nl;
+  if (by_k || by_p) {
+    hist_clear(S);
+    constexpr int U = 4;
+    for (int i0 = tid; i0 < nl; i0 += kThreads * U) {
+      float x[U];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (v.x[j] >= bound && v.x[j] > kNegInf) {
+      for (int e = 0; e < U; ++e) {
+        const int i = i0 + e * kThreads;
+        x[e] = i < nl ? gm_elem(P.lmax, l0 + i, A.type) : kNegInf;
+      }
+#pragma unroll
+      for (int e = 0; e < U; ++e) {
+        const int bin = dist_bin(x[e], R);
+        if (bin < 0) continue;
+        if (by_k) {
+          atomicAdd(&S.cnt[bin], 1u);
+        } else {
+          // a little less than it weighs
+          const float w = x[e] == R.xmax ? 1.f : __builtin_amdgcn_exp2f((x[e] - R.xmax) * (float)inv * 1.44269504f) * 0.9999f;
+          atomicAdd(&S.cnt[bin], 1u);
+          atomicAdd(&S.mass[bin], (unsigned long long)(w * 0x1p40f));
+        }
+      }
+    }
+    const double want = (double)rp.top_p * all;
+    hist_find(S, by_k, (unsigned long long)rp.top_k, want, 0x1p40);
+    const bool reached = by_k ? S.above_n + (int)S.cnt[S.bin] >= rp.top_k
+                              : (double)(S.above + S.mass[S.bin]) >= want * 0x1p40;
+    if (reached) limit = S.bin;
+    __syncthreads();
+  }
+  if (by_min && !(by_k && by_p)) {
+    // one bin more than the threshold's: the test itself is the weight's
+    const double d = -log((double)rp.min_p) * (double)kBinsPerE + 1.0;
+    if (d < (double)limit) limit = (int)d;
+  }
+  // ---- few candidates: ranked in LDS
+  if (limit < kBins - 1) {
+    int* const list = reinterpret_cast<int*>(S.mass);                    // kList of them
+    if (tid == 0) S.bin = 0;
+    __syncthreads();
+    constexpr int U = 4;
+    for (int i0 = tid; i0 < nl; i0 += kThreads * U) {
+      float x[U];
+#pragma unroll
+      for (int e = 0; e < U; ++e) {
+        const int i = i0 + e * kThreads;
+        x[e] = i < nl ? gm_elem(P.lmax, l0 + i, A.type) : kNegInf;
+      }
+#pragma unroll
+      for (int e = 0; e < U; ++e) {
+        const int bin = dist_bin(x[e], R);
+        if (bin < 0 || bin > limit) continue;
+        const int at = atomicAdd(&S.bin, 1);
+        if (at < kList) list[at] = i0 + e * kThreads;
+      }
+    }
+    __syncthreads();
+    const int nlist = S.bin;
+    if (nlist <= kList) {
+      for (int i = tid; i < nlist; i += kThreads) {
+        const Lane8 v = load8(P, row, list[i] >> 6, list[i] & 63);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int bin = dist_bin(v.x[j], R);
+          if (bin < 0 || bin > limit) continue;
           const int at = atomicAdd(&S.count, 1);
           if (at < kCand) S.cand[at] = (unsigned long long)~key_of(v.x[j]) << 32 | (uint32_t)v.at(j);
         }
+      }
     }
     __syncthreads();
-    const int n = S.count;
+    const int n = nlist <= kList ? S.count : kCand + 1;
     if (n <= kCand) {
       const unsigned long long mine = tid < n ? S.cand[tid] : 0;
-      const double w = tid < n ? weight(value_of(mine), R.xmax, R.inv, S.tab) : 0.0;
+      const double w = tid < n ? weight(value_of(mine), R.xmax, R.units, S.tab) : 0.0;
       rank_candidates(S, n, mine, w);
       // from here on thread r has the candidate of rank r
       const bool in_k = tid < n && (!by_k || tid < rp.top_k);
@@ -643,34 +835,28 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(Smp P) {
   }
   // ---- many: the cut, then the kept weight of every group
   Cut c{0u, 0x7fffffff};
-  if (by_k) {
-    double tk;
-    c = find_cut(P, S, gmax, R, true, rp.top_k, 0.0, &tk);
-    if (by_p) {
-      double none;
-      c = find_cut(P, S, gmax, R, false, 0, (double)rp.top_p * tk, &none);
-    }
-  } else if (by_p) {
-    double none;
-    c = find_cut(P, S, gmax, R, false, 0, (double)rp.top_p * all, &none);
-  }
+  bool whole = false;
+  double tk;
+  if (by_k) c = find_cut(P, S, gmax, gs, ec, R, limit, true, rp.top_k, 0.0, minw, &tk, &whole);
+  if (by_p)
+    c = find_cut(P, S, gmax, gs, ec, R, limit, false, 0, (double)rp.top_p * (by_k ? tk : all), minw, &tk, &whole);
   const bool cut = by_k || by_p;
   auto kept_w = [&](float x, int i) {
     if (!(x > kNegInf) || (cut && !kept(x, i, c))) return 0.0;
-    const double w = weight(x, R.xmax, R.inv, S.tab);
+    const double w = weight(x, R.xmax, R.units, S.tab);
     return w >= minw ? w : 0.0;
   };
-  if (cut || by_min) {
-    for (int g = wave; g < P.ng; g += kWaves) {
+  if ((cut && !whole) || (!cut && by_min)) {
+    for (int g = tid; g < P.ng; g += kThreads) gs[g] = 0.0;
+    __syncthreads();
+    each_group(P, gmax, R, limit, [&](int g, const Lane8& v) {
+      if (cut && key_of(gmax[g]) < c.key) return;
       double s = 0.0;
-      if (gmax[g] > kNegInf && (!cut || key_of(gmax[g]) >= c.key)) {
-        const Lane8 v = load8(P, row, g);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s += kept_w(v.x[j], v.at(j));
-        s = wave_sum(s);
-      }
+      for (int j = 0; j < 8; ++j) s += kept_w(v.x[j], v.at(j));
+      s = wave_sum(s);
       if (lane == 0) gs[g] = s;
-    }
+    });
     __syncthreads();
   }
   // the group where the running weight passes u times the total
@@ -742,19 +928,22 @@ int groups(const gm_sample_args* a) { return (a->vocab + kGroup - 1) / kGroup; }
 
 size_t gm_sample_ws(const gm_sample_args* a) {
   const size_t n = (size_t)a->n_row * groups(a);
-  return align256(n * 8) + align256(n * 4);
+  return align256(n * 8) + align256(n * 4) + align256(n * 64 * gm_elem_bytes(a->type));
 }
 
 int gm_sample_run(const gm_sample_args* a, uint8_t* ws, hipStream_t s) {
   Smp P{};
   P.a = *a;
   P.ng = groups(a);
+  const size_t n = (size_t)a->n_row * P.ng;
   P.gsum = reinterpret_cast<double*>(ws);
-  P.gmax = reinterpret_cast<float*>(ws + align256((size_t)a->n_row * P.ng * 8));
+  P.gmax = reinterpret_cast<float*>(ws + align256(n * 8));
+  P.lmax = ws + align256(n * 8) + align256(n * 4);
   P.vec = gm_rows_aligned(a->logits, a->type, a->row_stride, 0);
-  k_sample_groups<<<dim3((P.ng + 15) / 16, a->n_row), 256, 0, s>>>(P);
+  if (a->n_row >= 8) k_sample_groups<4><<<dim3((P.ng + 15) / 16, a->n_row), 256, 0, s>>>(P);
+  else k_sample_groups<1><<<dim3((P.ng + 3) / 4, a->n_row), 256, 0, s>>>(P);
   GM_TRY(hipGetLastError());
-  const size_t lds = sizeof(Shared) + (size_t)P.ng * 12;
+  const size_t lds = sizeof(Shared) + (size_t)P.ng * 16;
   if (int rc = gm_set_smem(k_sample_pick, lds)) return rc;
   k_sample_pick<<<a->n_row, kThreads, lds, s>>>(P);
   GM_TRY(hipGetLastError());
