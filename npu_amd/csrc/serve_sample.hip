@@ -15,12 +15,19 @@
 //                   total, or by min-p itself.  Only lanes with a maximum that near are
 //                   read again, and up to kCand candidates are ranked against each
 //                   other in LDS.  More than that (a flat nucleus, a large k): the same
-//                   histogram over all values finds the bin where the filter ends, and
-//                   only that bin's are ranked (or cut bit by bit, if they too are many).
+//                   histogram over all values.  Its weights are fp32 in fixed point, with
+//                   a bound on their error, so that it leaves an interval of bins (nearly
+//                   always one) that holds the end of the filter; one pass in 64 bits sums
+//                   what lies above, and only the interval's values are ranked (or cut
+//                   digit by digit of their bits, if they too are many).
 // Kept tokens run in the vocabulary's order, so nothing is ever sorted as a whole.
 // No result depends on the order of atomics: they count, or add fixed-point values.
 // Bound: HBM and, without top-k, the fp64 exponentials of the first kernel; for few
-// rows the second kernel's chain of block-wide steps.
+// rows the second kernel's chain of block-wide steps, for many flat rows its two passes.
+//
+// Measured, first and second kernel: one row of 248,320 fp32 with all filters 3 + 22 us;
+// 64 rows of 248,320 bf16 with mixed filters 20 + 31 us; 256 rows of 248,320 bf16 and their
+// nuclei of up to half the vocabulary 67 us (1.9 TB/s, beside its 64 M exponentials) + 232.
 #include "kernels.h"
 #include "serving.h"
 
@@ -28,9 +35,10 @@ namespace {
 
 constexpr int kGroup = 512;         // logits of a group: 8 per lane of a wave
 constexpr int kCand = 1024;         // candidates ranked in LDS, one per thread
-constexpr int kBins = 2048;         // bins of the distance from the maximum ...
-constexpr float kBinsPerE = 32.f;   // ... 1/32 wide, in units of the temperature
-constexpr int kList = 4096;         // lanes of 8 logits that are read again
+constexpr int kBins = 4096;         // bins of the distance from the maximum ...
+constexpr int kFine = 2048;         // ... these 1/128 wide in units of the temperature, the
+constexpr float kBinsPerE = 128.f;  // others 1/8: the ranges end 16 and 272 away
+constexpr int kList = 8192;         // lanes of 8 logits that are read again
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kPosInf = __builtin_inff();
 
@@ -268,8 +276,9 @@ __device__ __forceinline__ int block_min(int v, int* red) {
   return m;
 }
 
-__device__ __forceinline__ int block_max_u(uint32_t v, int* red) {
-  return (int)~(uint32_t)(block_min((int)(~v ^ 0x80000000u), red) ^ 0x80000000u);
+// The least of unsigned values.
+__device__ __forceinline__ uint32_t block_min_u(uint32_t v, int* red) {
+  return (uint32_t)block_min((int)(v ^ 0x80000000u), red) ^ 0x80000000u;
 }
 
 // Running sum over the threads, the own value with it; all: the sum.
@@ -294,10 +303,15 @@ __device__ __forceinline__ T block_scan(T v, T* red, T* all) {
   return v + before;
 }
 
-// Floats as integers of the same order.
-__device__ __forceinline__ uint32_t key_of(float x) {
+// Floats as integers of the same order, without the bits that the logits' type does
+// not have (low: 0 for fp32, 16 for bf16, 13 for fp16).
+__device__ __forceinline__ uint32_t key_of(float x, int low) {
   const uint32_t b = __float_as_uint(x);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  return (b & 0x80000000u ? ~b : b | 0x80000000u) >> low;
+}
+__device__ __forceinline__ float value_of(uint32_t key, int low) {
+  const uint32_t k = key << low;
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~(k | ((1u << low) - 1)));
 }
 
 struct Shared {
@@ -307,14 +321,13 @@ struct Shared {
   float fred[kWaves];
   int ired[kWaves];
   int count;
-  int bin;
+  int lo, hi;                           // of hist_find
+  int group, nth, id_of;                // of the equals at a cut
   unsigned long long above;
-  int above_n;
   unsigned long long cand[kCand];       // descending value, then index: (~key << 32) | index
   double w[kCand];
   int id[kCand];
-  unsigned long long mass[kBins];       // fixed point
-  unsigned int cnt[kBins];
+  unsigned long long mass[kBins];       // fixed point, or counts
 };
 
 static_assert(sizeof(Shared::mass) >= kList * sizeof(int));
@@ -325,21 +338,21 @@ struct Cut {
   uint32_t key;
   int id;
 };
-__device__ __forceinline__ bool kept(float x, int i, const Cut& c) {
-  const uint32_t k = key_of(x);
+__device__ __forceinline__ bool kept(float x, int i, const Cut& c, int low) {
+  const uint32_t k = key_of(x, low);
   return k > c.key || (k == c.key && i <= c.id);
 }
 
 struct Row {
-  int row;
+  int row, low;
   float xmax;
   float per_bin;     // bins per unit of x
+  float octaves;     // powers of two per unit of x
   double units;
-  double fix;        // fixed point of the histogram's masses: the sum of all fits 63 bits
 };
 
-// The thread's candidate (tid < n) among S.cand, ranked: its weight goes to S.w and
-// its entry's index to S.id at its rank.  Returns its rank.
+// The candidate `mine` of thread tid < n among S.cand[0 .. n), ranked: its weight goes to
+// S.w and its index to S.id at its rank.  Returns its rank.
 __device__ __forceinline__ int rank_candidates(Shared& S, int n, unsigned long long mine, double w) {
   int rank = 0;
   if ((int)threadIdx.x < n) {
@@ -351,91 +364,96 @@ __device__ __forceinline__ int rank_candidates(Shared& S, int n, unsigned long l
   return rank;
 }
 
-__device__ __forceinline__ float value_of(unsigned long long c) {
-  const uint32_t k = ~(uint32_t)(c >> 32);
-  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
-}
-
-// Adds a wave's lanes to S.cnt[bin] and S.mass[bin] (bin < 0: none).  Lanes that
-// all have one bin add once.
-__device__ __forceinline__ void hist_add(Shared& S, int bin, unsigned long long m) {
-  const unsigned long long on = __ballot(bin >= 0);
-  if (on == 0) return;
-  const int first = __shfl(bin, __ffsll(on) - 1, 64);
-  if (__ballot(bin >= 0 && bin != first) == 0) {
-    unsigned long long s = bin >= 0 ? m : 0;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    if ((threadIdx.x & 63) == 0) {
-      atomicAdd(&S.cnt[first], (unsigned)__popcll(on));
-      atomicAdd(&S.mass[first], s);
-    }
-  } else if (bin >= 0) {
-    atomicAdd(&S.cnt[bin], 1u);
-    atomicAdd(&S.mass[bin], m);
-  }
-}
+// The last bin has no end, and a row may have most of its values there: it is not counted,
+// but marked as one that reaches whatever is looked for.
+constexpr unsigned long long kMark = 1ull << 62;
 
 __device__ __forceinline__ void hist_clear(Shared& S) {
   __syncthreads();
-  for (int i = threadIdx.x; i < kBins; i += kThreads) {
-    S.cnt[i] = 0;
-    S.mass[i] = 0;
-  }
+#pragma unroll
+  for (int i = 0; i < kBins / kThreads; ++i) S.mass[threadIdx.x + i * kThreads] = 0;
   __syncthreads();
 }
 
-// The bin (bin 0 holds the largest values) where the running count reaches `k`
-// (by_count) or the running mass `m`: S.bin, with what lies before it in S.above,
-// S.above_n.  The last bin that holds anything where it is never reached.
-__device__ __forceinline__ void hist_find(Shared& S, bool by_count, unsigned long long k, double m, double fix) {
+// S.lo, S.hi: the bins (bin 0 holds the largest values) where the running mass reaches
+// tlo and thi, 0 < tlo <= thi; S.above: the mass before S.lo.  Where tlo is never reached
+// S.lo is the last bin that holds anything, and where thi is not S.hi is kBins.
+__device__ __forceinline__ void hist_find(Shared& S, unsigned long long tlo, unsigned long long thi) {
   constexpr int PER = kBins / kThreads;
   __syncthreads();
-  unsigned long long c[PER], s[PER], cs = 0, ss = 0, all;
+  unsigned long long c[PER], own = 0, all;
+  int last = -1;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    c[j] = S.cnt[threadIdx.x * PER + j];
-    s[j] = S.mass[threadIdx.x * PER + j];
-    cs += c[j];
-    ss += s[j];
+    c[j] = S.mass[threadIdx.x * PER + j];
+    own += c[j];
+    if (c[j]) last = threadIdx.x * PER + j;
   }
-  unsigned long long nb = block_scan<unsigned long long>(cs, S.ured, &all) - cs;
-  unsigned long long sb = block_scan<unsigned long long>(ss, S.ured, &all) - ss;
-  int hit = kBins, last = -1;
+  if (threadIdx.x == 0) {
+    S.lo = 0;
+    S.hi = kBins;
+    S.above = 0;
+  }
+  unsigned long long before = block_scan<unsigned long long>(own, S.ured, &all) - own;
+  const int end = -block_min(-last, S.ired);            // two barriers behind the clear above
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    const unsigned long long nn = nb + c[j], sn = sb + s[j];
-    const bool reach = by_count ? nn >= k : (double)sn >= m * fix;
-    if (c[j]) {
-      if (reach && hit == kBins) hit = threadIdx.x * PER + j;
-      last = threadIdx.x * PER + j;
+    const int bin = threadIdx.x * PER + j;
+    const unsigned long long after = before + c[j];
+    if ((before < tlo && after >= tlo) || (all < tlo && bin == end)) {
+      S.lo = bin;
+      S.above = before;
     }
-    nb = nn;
-    sb = sn;
-  }
-  int bin = block_min(hit, S.ired);
-  if (bin == kBins) bin = -block_min(-last, S.ired);
-  if (bin / PER == (int)threadIdx.x) {
-    // back to what lies before the bin
-#pragma unroll
-    for (int j = PER - 1; j >= 0; --j)
-      if ((int)threadIdx.x * PER + j >= bin) {
-        nb -= c[j];
-        sb -= s[j];
-      }
-    S.bin = bin;
-    S.above = sb;
-    S.above_n = (int)nb;
+    if (before < thi && after >= thi) S.hi = bin;
+    before = after;
   }
   __syncthreads();
 }
 
-// The bin of a value by its distance from the maximum; it never falls as x does.
+// The bin of a value by its distance from the maximum; it never falls as x does.  Top-k
+// with a low temperature ends far out: with all bins 1/128 wide, 64 rows with a 300th
+// value 33 temperatures away took 750 us instead of 50.
 __device__ __forceinline__ int dist_bin(float x, const Row& R) {
   if (!(x > kNegInf)) return -1;
   if (x == R.xmax) return 0;
   const float d = (R.xmax - x) * R.per_bin;
-  return d < (float)(kBins - 1) ? (int)d : kBins - 1;
+  const float b = d < (float)kFine ? d : (float)kFine + (d - (float)kFine) * (1.f / 16);
+  return b < (float)(kBins - 1) ? (int)b : kBins - 1;
+}
+
+// A weight in fp32 as a multiple of 2^-32, rounded down.  The exponent's rounding is the
+// largest of its errors: 2^-24 of up to 32 (smaller weights are 0), thrice, is 6e-6 of the
+// weight.  kHigh and kLow below leave 3e-5 for it, and one unit per value for the rounding
+// down.
+__device__ __forceinline__ unsigned long long mass_of(float x, const Row& R) {
+  const float w = x == R.xmax ? 1.f : __builtin_amdgcn_exp2f((x - R.xmax) * R.octaves);
+  return (unsigned long long)__float2uint_rz(fmaxf(w, 0.f) * 4294967040.f);
+}
+constexpr double kHigh = 1.0 + 0x1p-15, kLow = 1.0 - 0x1p-15;
+
+// f(index, maximum) for the lanes' maxima, 16 of a thread loaded together.
+template <typename F>
+__device__ __forceinline__ void each_max(const Smp& P, int row, F f) {
+  constexpr int U = 4;
+  const int n = P.ng * 16;                              // fours of them
+  const int64_t l0 = (int64_t)row * P.ng * 64;
+  for (int i0 = threadIdx.x; i0 < n; i0 += kThreads * U) {
+    float x[U][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * kThreads;
+      if (i < n) {
+        gm_load<4>(P.lmax, l0 + (int64_t)i * 4, P.a.type, true, x[u]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[u][e] = kNegInf;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f((i0 + u * kThreads) * 4 + e, x[u][e]);
+  }
 }
 
 // For the groups of this wave that may hold something of bin `limit` or nearer, four
@@ -458,83 +476,90 @@ __device__ __forceinline__ void each_group(const Smp& P, const float* gmax, cons
   }
 }
 
-// The cut at the k-th value (by_count) or where the running weight, from the
-// largest on, reaches m; *total: the weight of what is kept.  gs[g]: group g's kept
-// weight of at least minw; *whole: whether that is all of it, or what the bin of the
-// cut keeps is not in it yet.
-__device__ Cut find_cut(const Smp& P, Shared& S, const float* gmax, double* gs, int* ec, const Row& R, int limit,
-                        bool by_count, int k, double m, double minw, double* total, bool* whole) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+// The cut at the k-th value (by_count) or where the running weight, from the largest on,
+// reaches m, among the values of bin `limit` or nearer; all of those where neither
+// happens.  *total: the weight of what is kept.  gs[g]: group g's kept weight, of tokens
+// of at least minw; ec[g] is scratch.  All threads of the block call it.
+__device__ __forceinline__ Cut find_cut(const Smp& P, Shared& S, const float* gmax, double* gs, unsigned long long* ec,
+                                        const Row& R, int limit, bool by_count, int k, double m, double minw,
+                                        double* total) {
+  const int tid = threadIdx.x, lane = tid & 63;
   hist_clear(S);
+  bool far = false;
   each_group(P, gmax, R, limit, [&](int, const Lane8& v) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      int bin = dist_bin(v.x[j], R);
-      if (bin > limit) bin = -1;
-      unsigned long long w = 0;
-      if (bin >= 0 && !by_count) w = (unsigned long long)(weight(v.x[j], R.xmax, R.units, S.tab) * R.fix);
-      hist_add(S, bin, w);
+      const int bin = dist_bin(v.x[j], R);
+      if (bin == kBins - 1) far = true;
+      else if (bin >= 0 && bin <= limit) atomicAdd(&S.mass[bin], by_count ? 1ull : mass_of(v.x[j], R));
     }
   });
-  hist_find(S, by_count, (unsigned long long)k, m, R.fix);
-  const int bin = S.bin, members = (int)S.cnt[bin], above_n = S.above_n;
-  // the groups' weight above the bin in 64 bits, and the bin's members: how many a group
-  // has, their least and largest key, and themselves if they are few
-  if (threadIdx.x == 0) S.count = 0;
-  for (int g = threadIdx.x; g < P.ng; g += kThreads) {
+  if (far && limit == kBins - 1) S.mass[kBins - 1] = kMark;
+  if (by_count) {
+    hist_find(S, (unsigned long long)k, (unsigned long long)k);
+  } else {
+    const double lo = m * (0x1p32 / kHigh) - (double)P.a.vocab - 1.0, hi = m * (0x1p32 / kLow) + 1.0;
+    hist_find(S, (unsigned long long)fmax(lo, 1.0), (unsigned long long)fmax(hi, 1.0));
+  }
+  const int lo = S.lo, hi = min(max(S.hi, lo), limit);
+  const int above_n = by_count ? (int)S.above : 0;
+  // the weight above the interval in 64 bits, and its members: how many, their least and
+  // largest key, and themselves if they are few
+  if (tid == 0) S.count = 0;
+  for (int g = tid; g < P.ng; g += kThreads) {
     gs[g] = 0.0;
     ec[g] = 0;
   }
   __syncthreads();
   double sum = 0.0;
   uint32_t least = 0xffffffffu, most = 0u;
-  each_group(P, gmax, R, bin, [&](int g, const Lane8& v) {
+  each_group(P, gmax, R, hi, [&](int g, const Lane8& v) {
     double own = 0.0;
-    int e = 0;
+    const bool room = *static_cast<volatile int*>(&S.count) <= kCand;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int b = dist_bin(v.x[j], R);
-      if (b >= 0 && b < bin) {
+      if (b < 0 || b > hi) continue;
+      if (b < lo) {
         const double w = weight(v.x[j], R.xmax, R.units, S.tab);
         sum += w;
         own += w >= minw ? w : 0.0;
-      }
-      if (b == bin) {
-        const uint32_t key = key_of(v.x[j]);
+      } else {
+        const uint32_t key = key_of(v.x[j], R.low);
         least = min(least, key);
         most = max(most, key);
-        ++e;
-        if (members <= kCand) S.cand[atomicAdd(&S.count, 1)] = (unsigned long long)~key << 32 | (uint32_t)v.at(j);
+        const int at = room ? atomicAdd(&S.count, 1) : kCand;      // past kCand their number has no use
+        if (at < kCand) S.cand[at] = (unsigned long long)~key << 32 | (uint32_t)v.at(j);
       }
     }
     own = wave_sum(own);
-    e = gm_wave_sum(e);
-    if (lane == 0) {
-      gs[g] = own;
-      ec[g] = e;
-    }
+    if (lane == 0) gs[g] = own;
   });
   double above;
   block_scan<double>(sum, S.dred, &above);
-  least = ~(uint32_t)block_max_u(~least, S.ired);
-  most = (uint32_t)block_max_u(most, S.ired);
+  least = block_min_u(least, S.ired);
+  most = ~block_min_u(~most, S.ired);
+  const int members = S.count;
   Cut c;
-  *whole = false;
-  if (least != most && members <= kCand) {
-    __syncthreads();
-    const unsigned long long mine = (int)threadIdx.x < members ? S.cand[threadIdx.x] : 0;
-    const double w = (int)threadIdx.x < members ? weight(value_of(mine), R.xmax, R.units, S.tab) : 0.0;
+  if (members <= kCand) {
+    const unsigned long long mine = tid < members ? S.cand[tid] : 0;
+    const double w = tid < members ? weight(value_of(~(uint32_t)(mine >> 32), R.low), R.xmax, R.units, S.tab) : 0.0;
     const int rank = rank_candidates(S, members, mine, w);
+    // from here on thread r has the candidate of rank r
     double all;
-    const double ws = (int)threadIdx.x < members ? S.w[threadIdx.x] : 0.0;
-    const double run = block_scan<double>(ws, S.dred, &all);                 // thread r: rank r
-    const bool in = (int)threadIdx.x < members &&
-                    (by_count ? above_n + (int)threadIdx.x < k : threadIdx.x == 0 || above + (run - ws) < m);
+    const double ws = tid < members ? S.w[tid] : 0.0;
+    const double run = block_scan<double>(ws, S.dred, &all);
+    const bool in = tid < members && (by_count ? above_n + tid < k : tid == 0 || above + (run - ws) < m);
     int n;
     block_scan<int>(in ? 1 : 0, S.ired, &n);
     if (n < 1) n = 1;
-    if ((int)threadIdx.x == n - 1) S.w[0] = above + run;
-    if ((int)threadIdx.x < members && rank == n - 1) S.cand[0] = mine;
+    // a group's kept members in multiples of 2^-54 of the largest weight: 512 of them fit
+    if (tid < n && tid < members && ws >= minw)
+      atomicAdd(&ec[S.id[tid] / kGroup], (unsigned long long)__double2ull_rz(ws * 0x1p54));
+    __syncthreads();
+    if (tid == n - 1) S.w[0] = above + run;
+    if (tid < members && rank == n - 1) S.cand[0] = mine;
+    for (int g = tid; g < P.ng; g += kThreads) gs[g] += (double)ec[g] * 0x1p-54;
     __syncthreads();
     c.key = ~(uint32_t)(S.cand[0] >> 32);
     c.id = (int)(uint32_t)S.cand[0];
@@ -542,124 +567,120 @@ __device__ Cut find_cut(const Smp& P, Shared& S, const float* gmax, double* gs, 
     __syncthreads();
     return c;
   }
-  // many members, or equals: the keys' distance from the largest in digits of 11 bits
-  // (none if all are one value; 16-bit logits leave the low bits of a key alone)
-  const int low = P.a.type == GM_QTYPE_F32 ? 0 : P.a.type == GM_QTYPE_BF16 ? 16 : 13;
-  const uint32_t span = (most - least) >> low;
-  double over = above;                                  // weight above what is left
-  int over_n = above_n, equal = members;
-  uint32_t gap = 0, known = 0;                          // settled digits of the gap, and their mask
-  for (int top = 32 - __clz(span | 1) - (span == 0); top > 0;) {
-    const int bits = top < 11 ? top : 11, shift = top - bits;
+  // many members: their keys' distance from the largest in digits of 12 bits, 3 of them
+  // at most (none if all are one value)
+  const uint32_t span = most - least;
+  const double top_w = weight(value_of(most, R.low), R.xmax, R.units, S.tab);
+  // fixed point for the members' weights: top_w below 2^(62 - the vocabulary's bits)
+  const int up = 62 - (32 - __clz(P.a.vocab)) - (top_w > 0.0 ? ilogb(top_w) + 1 : 0);
+  const double fix = ldexp(1.0, up);
+  unsigned long long left = by_count ? (unsigned long long)max(k - above_n, 1)
+                                     : (unsigned long long)fmin(fmax((m - above) * fix, 1.0), 0x1p62);
+  uint32_t gap = 0, known = 0;                          // settled digits of the distance, and their mask
+  int top = span ? 32 - __clz(span) : 0;
+  for (int digit = 0; digit < 3; ++digit) {
+    if (top == 0) break;
+    const int bits = min(top, 12), shift = top - bits;
+    const uint32_t mask = (1u << bits) - 1;
     hist_clear(S);
-    each_group(P, gmax, R, bin, [&](int, const Lane8& v) {
+    each_group(P, gmax, R, hi, [&](int, const Lane8& v) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint32_t d = (most - key_of(v.x[j])) >> low;
-        const bool on = dist_bin(v.x[j], R) == bin && (d & known) == gap;
-        unsigned long long w = 0;
-        if (on && !by_count) w = (unsigned long long)(weight(v.x[j], R.xmax, R.units, S.tab) * R.fix);
-        hist_add(S, on ? (int)(d >> shift & ((1u << bits) - 1)) : -1, w);
+        const int b = dist_bin(v.x[j], R);
+        if (b < lo || b > hi) continue;                 // lo >= 0
+        const uint32_t d = most - key_of(v.x[j], R.low);
+        if ((d & known) != gap) continue;
+        const unsigned long long one =
+            by_count ? 1ull : __double2ull_rz(weight(v.x[j], R.xmax, R.units, S.tab) * fix);
+        atomicAdd(&S.mass[d >> shift & mask], one);
       }
     });
-    hist_find(S, by_count, by_count ? (unsigned long long)(k - over_n) : 0, m - over, R.fix);
-    over_n += S.above_n;
-    equal = (int)S.cnt[S.bin];
-    gap |= (uint32_t)S.bin << shift;
-    known |= ((1u << bits) - 1) << shift;
+    hist_find(S, left, left);
+    left = left > S.above ? left - S.above : 1;
+    gap |= (uint32_t)S.lo << shift;
+    known |= mask << shift;
     top = shift;
-    // the weight above in 64 bits: values of the settled digits nearer than this one
-    double part = 0.0;
-    const uint32_t g1 = gap, kn = known, sh = (uint32_t)shift;
-    if (by_count) {
-      // only wanted at the end, where it is formed from the cut itself
-    } else {
-      each_group(P, gmax, R, bin, [&](int, const Lane8& v) {
+    __syncthreads();
+  }
+  c.key = most - gap;
+  // the members above the cut's value in 64 bits, and how many every group has of it
+  double part = 0.0, more;
+  int near = 0, near_all;
+  each_group(P, gmax, R, hi, [&](int g, const Lane8& v) {
+    double own = 0.0;
+    int e = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t d = (most - key_of(v.x[j])) >> low;
-          const uint32_t before = kn & ~(((1u << bits) - 1) << sh);
-          if (dist_bin(v.x[j], R) == bin && (d & before) == (g1 & before) && (d & kn) < g1)
-            part += weight(v.x[j], R.xmax, R.units, S.tab);
-        }
-      });
+    for (int j = 0; j < 8; ++j) {
+      const int b = dist_bin(v.x[j], R);
+      if (b < lo || b > hi) continue;
+      const uint32_t key = key_of(v.x[j], R.low);
+      if (key > c.key) {
+        const double w = weight(v.x[j], R.xmax, R.units, S.tab);
+        part += w;
+        own += w >= minw ? w : 0.0;
+        ++near;
+      }
+      e += key == c.key ? 1 : 0;
     }
-    double more;
-    block_scan<double>(part, S.dred, &more);
-    over += more;
-    __syncthreads();
+    own = wave_sum(own);
+    e = gm_wave_sum(e);
+    if (lane == 0) {
+      gs[g] += own;
+      ec[g] = (unsigned long long)e;
+    }
+  });
+  block_scan<double>(part, S.dred, &more);
+  block_scan<int>(near, S.ired, &near_all);
+  // the nth index that holds the cut's value: the groups in order, every thread some
+  const int per = (P.ng + kThreads - 1) / kThreads, g0 = min(tid * per, P.ng), g1 = min(g0 + per, P.ng);
+  int own = 0, equal;
+  for (int g = g0; g < g1; ++g) own += (int)ec[g];
+  int run = block_scan<int>(own, S.ired, &equal) - own;
+  const double w1 = weight(value_of(c.key, R.low), R.xmax, R.units, S.tab);
+  const double over = above + more;
+  const double need = by_count ? (double)(k - above_n - near_all) : w1 > 0.0 ? ceil((m - over) / w1) : (double)equal;
+  const int nth = max((int)fmin(need, (double)equal), 1);
+  *total = over + (double)nth * w1;
+  if (tid == 0) {
+    S.group = 0;
+    S.nth = 0;
+    S.id_of = 0x7fffffff;
   }
-  c.key = most - (gap << low);
-  if (by_count && span) {
-    // the weight of the bin's values above the cut's
-    double part = 0.0, more;
-    each_group(P, gmax, R, bin, [&](int, const Lane8& v) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (dist_bin(v.x[j], R) == bin && key_of(v.x[j]) > c.key) part += weight(v.x[j], R.xmax, R.units, S.tab);
-    });
-    block_scan<double>(part, S.dred, &more);
-    over += more;
-  }
-  const float x = value_of((unsigned long long)~c.key << 32);
-  const double w1 = weight(x, R.xmax, R.units, S.tab);
-  double need = by_count ? (double)(k - over_n) : w1 > 0.0 ? ceil((m - over) / w1) : (double)equal;
-  need = fmin(fmax(need, 1.0), (double)equal);
-  const int nth = (int)need;
-  *total = over + need * w1;
-  if (span) {
-    // how many of exactly this value every group has
-    __syncthreads();
-    each_group(P, gmax, R, bin, [&](int g, const Lane8& v) {
-      int e = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) e += v.x[j] > kNegInf && key_of(v.x[j]) == c.key ? 1 : 0;
-      e = gm_wave_sum(e);
-      if (lane == 0) ec[g] = e;
-    });
-    __syncthreads();
-  }
-  // the nth index that holds x: the groups in order, every thread some
-  const int per = (P.ng + kThreads - 1) / kThreads, g0 = min((int)threadIdx.x * per, P.ng), g1 = min(g0 + per, P.ng);
-  int own = 0, all;
-  for (int g = g0; g < g1; ++g) own += ec[g];
-  int run = block_scan<int>(own, S.ired, &all) - own;
+  __syncthreads();
   for (int g = g0; g < g1; ++g) {
-    const int e = ec[g], in = min(max(nth - run, 0), e);
-    if (e > 0 && in > 0 && run + e >= nth) {             // the group of the nth
-      S.bin = g;
-      S.above_n = nth - run;
+    const int e = (int)ec[g], in = min(max(nth - run, 0), e);
+    if (in > 0 && run + e >= nth) {                      // the group of the nth
+      S.group = g;
+      S.nth = in;
     }
     if (w1 >= minw) gs[g] += (double)in * w1;
     run += e;
   }
   __syncthreads();
-  *whole = span == 0;
-  if (wave == 0) {
-    const Lane8 v = load8(P, R.row, S.bin);
-    // the group's equals in index order, one after the other
-    int left = S.above_n, at = -1;
-    uint32_t mine = 0;
+  if (tid < 64) {
+    const Lane8 v = load8(P, R.row, S.group);
+    const int want = S.nth, w8 = P.a.type == GM_QTYPE_F32 ? 4 : 8;
+    int before = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) mine |= (v.x[j] > kNegInf && key_of(v.x[j]) == c.key ? 1u : 0u) << j;
-    while (left > 0) {
-      int best = 0x7fffffff;
+    for (int h = 0; h < 2; ++h) {                        // index order: lanes, then their fours of fp32's second half
+      int mine = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) mine += j / w8 == h && v.x[j] > kNegInf && key_of(v.x[j], R.low) == c.key ? 1 : 0;
+      int inc = mine;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int other = __shfl_up(inc, o, 64);
+        if (lane >= o) inc += other;
+      }
+      int at = before + inc - mine;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (mine >> j & 1) best = min(best, v.at(j));
-      int first = best;
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) first = min(first, __shfl_xor(first, o, 64));
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (v.at(j) == first) mine &= ~(1u << j);
-      at = first;
-      --left;
+        if (j / w8 == h && v.x[j] > kNegInf && key_of(v.x[j], R.low) == c.key && ++at == want) S.id_of = v.at(j);
+      before += __shfl(inc, 63, 64);
     }
-    if (threadIdx.x == 0) S.count = at;
   }
   __syncthreads();
-  c.id = S.count;
+  c.id = S.id_of;
   __syncthreads();
   return c;
 }
@@ -667,9 +688,9 @@ __device__ Cut find_cut(const Smp& P, Shared& S, const float* gmax, double* gs, 
 __global__ void __launch_bounds__(kThreads) k_sample_pick(Smp P) {
   extern __shared__ __attribute__((aligned(16))) char dyn[];
   Shared& S = *reinterpret_cast<Shared*>(dyn);
-  double* gs = reinterpret_cast<double*>(dyn + sizeof(Shared));          // [ng]
-  float* gmax = reinterpret_cast<float*>(gs + P.ng);                     // [ng]
-  int* ec = reinterpret_cast<int*>(gmax + P.ng);                         // [ng]
+  double* gs = reinterpret_cast<double*>(dyn + sizeof(Shared));                 // [ng]
+  unsigned long long* ec = reinterpret_cast<unsigned long long*>(gs + P.ng);    // [ng]
+  float* gmax = reinterpret_cast<float*>(ec + P.ng);                            // [ng]
   const gm_sample_args& A = P.a;
   const int row = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   exp_table(S.tab);
@@ -682,11 +703,12 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(Smp P) {
   if (tid == 0) S.count = 0;
   Row R;
   R.row = row;
+  R.low = A.type == GM_QTYPE_F32 ? 0 : A.type == GM_QTYPE_BF16 ? 16 : 13;
   R.xmax = block_max(mx, S.fred);
   const double inv = 1.0 / (double)rp.t;
   R.units = kUnits / (double)rp.t;
   R.per_bin = (float)(inv * (double)kBinsPerE);
-  R.fix = ldexp(1.0, 62 - (32 - __clz(A.vocab)));
+  R.octaves = (float)(inv * 1.4426950408889634);
   if (R.xmax == kNegInf) {
     if (tid == 0) A.ids[row] = -1;
     return;
@@ -723,67 +745,37 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(Smp P) {
   const double u = (double)A.u[row];
   // ---- the farthest bin that may hold something kept, or counted by a filter before
   int limit = kBins - 1;
-  const int nl = P.ng * 64;
-  const int64_t l0 = (int64_t)row * nl;
   if (by_k || by_p) {
     hist_clear(S);
-    constexpr int U = 4;
-    for (int i0 = tid; i0 < nl; i0 += kThreads * U) {
-      float x[U];
-#pragma unroll
-      for (int e = 0; e < U; ++e) {
-        const int i = i0 + e * kThreads;
-        x[e] = i < nl ? gm_elem(P.lmax, l0 + i, A.type) : kNegInf;
-      }
-#pragma unroll
-      for (int e = 0; e < U; ++e) {
-        const int bin = dist_bin(x[e], R);
-        if (bin < 0) continue;
-        if (by_k) {
-          atomicAdd(&S.cnt[bin], 1u);
-        } else {
-          // a little less than it weighs
-          const float w = x[e] == R.xmax ? 1.f : __builtin_amdgcn_exp2f((x[e] - R.xmax) * (float)inv * 1.44269504f) * 0.9999f;
-          atomicAdd(&S.cnt[bin], 1u);
-          atomicAdd(&S.mass[bin], (unsigned long long)(w * 0x1p40f));
-        }
-      }
-    }
-    const double want = (double)rp.top_p * all;
-    hist_find(S, by_k, (unsigned long long)rp.top_k, want, 0x1p40);
-    const bool reached = by_k ? S.above_n + (int)S.cnt[S.bin] >= rp.top_k
-                              : (double)(S.above + S.mass[S.bin]) >= want * 0x1p40;
-    if (reached) limit = S.bin;
+    each_max(P, row, [&](int, float x) {
+      const int bin = dist_bin(x, R);
+      if (bin >= 0 && bin < kBins - 1) atomicAdd(&S.mass[bin], by_k ? 1ull : mass_of(x, R));
+    });
+    const unsigned long long want =
+        by_k ? (unsigned long long)rp.top_k : (unsigned long long)((double)rp.top_p * all * (0x1p32 / kLow)) + 1;
+    hist_find(S, want, want);
+    limit = min(limit, S.hi);
     __syncthreads();
   }
   if (by_min && !(by_k && by_p)) {
     // one bin more than the threshold's: the test itself is the weight's
-    const double d = -log((double)rp.min_p) * (double)kBinsPerE + 1.0;
-    if (d < (double)limit) limit = (int)d;
+    const double d = -log((double)rp.min_p) * (double)kBinsPerE;
+    const double b = (d < kFine ? d : kFine + (d - kFine) * (1.0 / 16)) + 1.0;
+    if (b < (double)limit) limit = (int)b;
   }
   // ---- few candidates: ranked in LDS
   if (limit < kBins - 1) {
     int* const list = reinterpret_cast<int*>(S.mass);                    // kList of them
-    if (tid == 0) S.bin = 0;
+    if (tid == 0) S.lo = 0;
     __syncthreads();
-    constexpr int U = 4;
-    for (int i0 = tid; i0 < nl; i0 += kThreads * U) {
-      float x[U];
-#pragma unroll
-      for (int e = 0; e < U; ++e) {
-        const int i = i0 + e * kThreads;
-        x[e] = i < nl ? gm_elem(P.lmax, l0 + i, A.type) : kNegInf;
-      }
-#pragma unroll
-      for (int e = 0; e < U; ++e) {
-        const int bin = dist_bin(x[e], R);
-        if (bin < 0 || bin > limit) continue;
-        const int at = atomicAdd(&S.bin, 1);
-        if (at < kList) list[at] = i0 + e * kThreads;
-      }
-    }
+    each_max(P, row, [&](int i, float x) {
+      const int bin = dist_bin(x, R);
+      if (bin < 0 || bin > limit) return;
+      const int at = atomicAdd(&S.lo, 1);
+      if (at < kList) list[at] = i;
+    });
     __syncthreads();
-    const int nlist = S.bin;
+    const int nlist = S.lo;
     if (nlist <= kList) {
       for (int i = tid; i < nlist; i += kThreads) {
         const Lane8 v = load8(P, row, list[i] >> 6, list[i] & 63);
@@ -792,7 +784,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(Smp P) {
           const int bin = dist_bin(v.x[j], R);
           if (bin < 0 || bin > limit) continue;
           const int at = atomicAdd(&S.count, 1);
-          if (at < kCand) S.cand[at] = (unsigned long long)~key_of(v.x[j]) << 32 | (uint32_t)v.at(j);
+          if (at < kCand) S.cand[at] = (unsigned long long)~key_of(v.x[j], R.low) << 32 | (uint32_t)v.at(j);
         }
       }
     }
@@ -800,7 +792,7 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(Smp P) {
     const int n = nlist <= kList ? S.count : kCand + 1;
     if (n <= kCand) {
       const unsigned long long mine = tid < n ? S.cand[tid] : 0;
-      const double w = tid < n ? weight(value_of(mine), R.xmax, R.units, S.tab) : 0.0;
+      const double w = tid < n ? weight(value_of(~(uint32_t)(mine >> 32), R.low), R.xmax, R.units, S.tab) : 0.0;
       rank_candidates(S, n, mine, w);
       // from here on thread r has the candidate of rank r
       const bool in_k = tid < n && (!by_k || tid < rp.top_k);
@@ -835,22 +827,20 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(Smp P) {
   }
   // ---- many: the cut, then the kept weight of every group
   Cut c{0u, 0x7fffffff};
-  bool whole = false;
-  double tk;
-  if (by_k) c = find_cut(P, S, gmax, gs, ec, R, limit, true, rp.top_k, 0.0, minw, &tk, &whole);
-  if (by_p)
-    c = find_cut(P, S, gmax, gs, ec, R, limit, false, 0, (double)rp.top_p * (by_k ? tk : all), minw, &tk, &whole);
   const bool cut = by_k || by_p;
+  double tk = all;
+#pragma nounroll
+  for (int f = by_k ? 0 : 1; f < (by_p ? 2 : 1); ++f)      // the k largest, then their nucleus
+    c = find_cut(P, S, gmax, gs, ec, R, limit, f == 0, rp.top_k, (double)rp.top_p * tk, minw, &tk);
   auto kept_w = [&](float x, int i) {
-    if (!(x > kNegInf) || (cut && !kept(x, i, c))) return 0.0;
+    if (!(x > kNegInf) || (cut && !kept(x, i, c, R.low))) return 0.0;
     const double w = weight(x, R.xmax, R.units, S.tab);
     return w >= minw ? w : 0.0;
   };
-  if ((cut && !whole) || (!cut && by_min)) {
+  if (!cut && by_min) {
     for (int g = tid; g < P.ng; g += kThreads) gs[g] = 0.0;
     __syncthreads();
     each_group(P, gmax, R, limit, [&](int g, const Lane8& v) {
-      if (cut && key_of(gmax[g]) < c.key) return;
       double s = 0.0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) s += kept_w(v.x[j], v.at(j));
@@ -879,7 +869,8 @@ __global__ void __launch_bounds__(kThreads) k_sample_pick(Smp P) {
     before = next;
   }
   const int first = block_min(hit, S.ired);
-  const int g = first != 0x7fffffff ? first : -block_min(-last, S.ired);
+  // a kept weight is somewhere: the maximum's is 1
+  const int g = first != 0x7fffffff ? first : max(-block_min(-last, S.ired), 0);
   if (hit == first && first != 0x7fffffff) S.w[0] = start;
   __syncthreads();
   if (wave > 0) return;
@@ -943,7 +934,7 @@ int gm_sample_run(const gm_sample_args* a, uint8_t* ws, hipStream_t s) {
   if (a->n_row >= 8) k_sample_groups<4><<<dim3((P.ng + 15) / 16, a->n_row), 256, 0, s>>>(P);
   else k_sample_groups<1><<<dim3((P.ng + 3) / 4, a->n_row), 256, 0, s>>>(P);
   GM_TRY(hipGetLastError());
-  const size_t lds = sizeof(Shared) + (size_t)P.ng * 16;
+  const size_t lds = sizeof(Shared) + (size_t)P.ng * 20;
   if (int rc = gm_set_smem(k_sample_pick, lds)) return rc;
   k_sample_pick<<<a->n_row, kThreads, lds, s>>>(P);
   GM_TRY(hipGetLastError());

@@ -544,6 +544,42 @@ def test_sample_rows_that_are_masked(gpu):
         assert got.tolist() == [_sample_ref(x[b], 0.5, _f32(t), k, _f32(p), _f32(mp)) for b in range(8)], (t, k, p, mp)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF, HF])
+@pytest.mark.parametrize("V", [4000, 131_072])
+def test_sample_flat_rows_of_both_signs(gpu, V, dtype):
+    """Thousands of values about 0 that are nearly equal in weight: the cut is found among
+    their bits, where the order of the negative ones is the other way round."""
+    g = _g(V)
+    flat = [(1.0, V // 2, 1.0, 0.0), (1.0, 0, 0.4, 0.0), (1.0, 3 * V // 4, 0.7, 0.0), (1.0, V - 1, 1.0, 0.0),
+            (1.0, 0, 1 - 2.0 ** -24, 0.0), (1.0, 0, 0.6, 0.9995), (1.0, 0, 1.0, 0.9995), (1e-4, 0, 0.9999, 0.0),
+            (1e-5, V // 3, 1.0, 0.0), (1e-4, V // 3, 0.9999, 1e-12), (1e-2, 0, 0.9999999, 0.0)]
+    x = _randn(g, len(flat), V, scale=1e-3).to(dtype)
+    u = torch.rand(len(flat), generator=g, device="cuda")
+    t, k, p, mp = (torch.tensor(c, dtype=d, device="cuda") for c, d in zip(zip(*flat), (F32, torch.int32, F32, F32)))
+    got = ops.sample(x, u, temperature=t, top_k=k, top_p=p, min_p=mp)
+    assert got.tolist() == [_sample_ref(x[b], float(u[b]), *(_f32(f) if i != 1 else f for i, f in enumerate(flat[b])))
+                            for b in range(len(flat))]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF, HF])
+def test_sample_filters_that_end_far_out(gpu, dtype):
+    """A few tokens far above all others: the k-th value is tens to thousands of temperatures
+    away, past the histogram's fine bins and past its last."""
+    g = _g(77)
+    V = 30_000
+    rows = [(t, k, p, mp) for t in (0.5, 0.2, 0.01) for k, p, mp in
+            ((40, 1.0, 0.0), (1500, 1.0, 0.0), (300, 0.999, 0.0), (0, 1 - 2.0 ** -24, 0.0), (0, 1.0, 1e-30), (5, 0.9, 0.5))]
+    x = _randn(g, len(rows), V, scale=2.0)
+    x[:, 17:V:4001] += 15.0
+    x = x.to(dtype)
+    u = torch.rand(len(rows), generator=g, device="cuda")
+    u[::2] = 1 - 2.0 ** -24
+    t, k, p, mp = (torch.tensor(c, dtype=d, device="cuda") for c, d in zip(zip(*rows), (F32, torch.int32, F32, F32)))
+    got = ops.sample(x, u, temperature=t, top_k=k, top_p=p, min_p=mp)
+    assert got.tolist() == [_sample_ref(x[b], float(u[b]), *(_f32(f) if i != 1 else f for i, f in enumerate(rows[b])))
+                            for b in range(len(rows))]
+
+
 # ------------------------------------------------------------ capture, a run of them together
 def test_captured_and_replayed_with_other_lengths(gpu):
     """A decode step of the four operators in a graph: replayed with other positions, lengths,
