@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(64 * NW, WPS) k_prompt_attn(Pmt P) {
   // p = 2^(score - reference + kStart) of the first tile's maximum (pass 0), kExact of the
   // row's (pass 2); a tile's p of a row sum to at most kMost
   constexpr bool F16 = QT == GM_QTYPE_F16;
-  constexpr float kStart = F16 ? 0.f : 0.f, kExact = F16 ? 14.f : 0.f, kMost = F16 ? 32768.f : 0x1p80f;
+  constexpr float kStart = 0.f, kExact = F16 ? 14.f : 0.f, kMost = F16 ? 32768.f : 0x1p80f;
   extern __shared__ __attribute__((aligned(1024))) char lds[];      // K [2][TILE], V [2][TILE], queries [NW][QL][1024]
   __shared__ int votes[NW];
   const gm_prompt_attn_args& A = P.a;

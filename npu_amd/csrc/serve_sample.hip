@@ -26,7 +26,7 @@
 // rows the second kernel's chain of block-wide steps, for many flat rows its two passes.
 //
 // Measured, first and second kernel: one row of 248,320 fp32 with all filters 3 + 22 us;
-// 64 rows of 248,320 bf16 with mixed filters 20 + 31 us; 256 rows of 248,320 bf16 and their
+// 64 rows of 248,320 fp32 with mixed filters 20 (3.2 TB/s) + 31 us; 256 rows of 248,320 bf16 and their
 // nuclei of up to half the vocabulary 67 us (1.9 TB/s, beside its 64 M exponentials) + 232.
 #include "kernels.h"
 #include "serving.h"

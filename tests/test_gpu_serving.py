@@ -412,6 +412,65 @@ def test_prompt_attention_scores_that_grow(gpu):
         _close(out, want, _tol(want, absv, v, dtype, dtype))
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("paged", [False, True])
+@pytest.mark.parametrize("hq,hkv,dh,new,cached,gate", [
+    (16, 2, 256, [1, 1500, 0, 2099, 600], [0, 70, 9, 1, 333], True),    # Dh 256 with enough rows for wide blocks
+    (20, 1, 256, [3300], [31], False),
+    (8, 2, 64, [i % 7 for i in range(100)], [(5 * i) % 41 for i in range(100)], False),     # over 64 sequences
+    (16, 2, 256, [(3 * i) % 40 for i in range(150)], [0] * 150, True),
+    (2, 2, 128, [0] * 70 + [300] + [0] * 70 + [129, 1], [0] * 143, False),
+])
+def test_prompt_attention_large(gpu, dtype, paged, hq, hkv, dh, new, cached, gate):
+    test_prompt_attention(gpu, dtype, paged, hq, hkv, dh, new, cached, gate)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("dh", [64, 256])
+def test_prompt_attention_queries_at_odd_elements(gpu, dtype, dh):
+    g = _g(16)
+    T = 77
+    row = _randn(g, T, 4, 2 * dh + 1, dtype=dtype)
+    q, gt = row[..., 1:dh + 1], row[..., dh + 1:]
+    k, v = (_randn(g, T, 2, dh, dtype=dtype) for _ in range(2))
+    cu = torch.tensor([0, T], dtype=torch.int32, device="cuda")
+    out = ops.prompt_attention(q, k, v, cu, gate=gt)
+    assert torch.equal(out, ops.prompt_attention(q.contiguous(), k, v, cu, gate=gt.contiguous()))
+    want, absv = _attend_ref(q, k, v, dh ** -0.5, torch.arange(T, device="cuda"))
+    f = torch.sigmoid(gt.double())
+    _close(out, want * f, _tol(want * f, absv * f, v, dtype, dtype))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_prompt_attention_wide_blocks_on_odd_values(gpu, dtype):
+    """The Dh 256 variant for many rows: values that are not finite behind and before a token,
+    and scores that grow with every key."""
+    g = _g(17)
+    T, hq = 4200, 16
+    q, k, v = (_randn(g, T, h, 256, dtype=dtype) for h in (hq, 2, 2))
+    cu = torch.tensor([0, T], dtype=torch.int32, device="cuda")
+    clean = ops.prompt_attention(q, k, v, cu)
+    at = 3001
+    v[at, 0, 3], v[at + 1, 1, 250] = float("inf"), float("nan")
+    k[at + 500, 1, 9] = float("nan")
+    out = ops.prompt_attention(q, k, v, cu)
+    assert torch.equal(out[:at], clean[:at])
+    h = hq // 2
+    assert bool((out[at:, :h, 3] == float("inf")).all()) and torch.equal(out[at:, :h, 4:], clean[at:, :h, 4:])
+    assert bool(out[at + 1:, h:, 250].isnan().all()) and bool(out[at + 500:, h:].isnan().all())
+    assert torch.equal(out[at + 1:at + 500, h:, :250], clean[at + 1:at + 500, h:, :250])
+    for top in (60.0, 30_000.0):
+        q = torch.zeros(T, hq, 256, dtype=dtype, device="cuda")
+        q[..., 0] = 1.0
+        k = _randn(g, T, 1, 256, dtype=dtype)
+        k[:, 0, 0] = torch.linspace(0, top, T, device="cuda").to(dtype)
+        v = _randn(g, T, 1, 256, dtype=dtype)
+        out = ops.prompt_attention(q, k, v, cu, scale=1.0)
+        want, absv = _attend_ref(q[:, :1], k, v, 1.0, torch.arange(T, device="cuda"))
+        _close(out[:, :1], want, _tol(want, absv, v, dtype, dtype))
+        assert torch.equal(out, out[:, :1].expand_as(out))
+
+
 def test_prompt_attention_one_token_is_paged_attention(gpu):
     """One query row per sequence: the two operators' results agree to their roundings."""
     g = _g(14)
