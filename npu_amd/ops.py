@@ -285,7 +285,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     q [T, n_head, head_dim], k and v [T, n_head_kv, head_dim] (one type; views into a
     projection's rows are fine); positions int32 [T] or [n_axes, T]; inv_freq fp64
     [rope_dim / 2], radians per position, and axis int32 [rope_dim / 2], the axis that turns
-    each pair (``qwen_core.build_rope_axes``); k_pages / v_pages [n_pages, page_size,
+    each pair (``qwen_serve.build_rope_axes``); k_pages / v_pages [n_pages, page_size,
     n_head_kv, head_dim] bf16 or fp16; slots int32 [T], the cache row of each token (page
     times page_size plus row), negative for none, no row twice.  The result has the cache's
     type, or ``out_dtype``.  A packed buffer [T, n_head_kv, head_dim] viewed as one page,
