@@ -22,7 +22,9 @@
 //                    then has row n = dim 8 n + i
 // so K and V pass from memory to the MFMAs without LDS, every byte once.
 // Bound: HBM; 32 keys of 256 dims (32 KB) cost a wave about 900 cycles of MFMA,
-// perm and softmax, a fifth of what the card's rate leaves it.
+// perm and softmax, a fifth of what the card's rate leaves it.  Measured, with the join:
+// 4 x 131,071 positions of 8 x 128 (2.1 GB) 356 us, 6.0 TB/s; 64 ragged ones up to 8,192 of
+// 2 x 256 84 us; one of 4,001 with fp32 queries 16 us, the latencies of two launches.
 //
 // fp32 queries (NP > 1): q and p go as NP planes of the cache's type (three of
 // bf16: exact; two of f16, q scaled to 2^9 .. 2^10 and p to 2^15: 22 bits).  The
@@ -80,11 +82,16 @@ __device__ __forceinline__ void scan_rounds(const Dec& P, int* pre, int* wsum) {
   __syncthreads();
 }
 
-// Four outputs of one head: o / l (0 where there was no key), times sigmoid(gate).
-__device__ __forceinline__ void write_out(const Dec& P, int b, int h, int d, gm_f32x4 o, float l) {
+__device__ __forceinline__ void load_gate(const Dec& P, int b, int h, int d, float (&g)[4]) {
   const gm_paged_attn_args& A = P.a;
-  float v[4], g[4] = {0.f, 0.f, 0.f, 0.f};
+  g[0] = g[1] = g[2] = g[3] = 0.f;
   if (A.gate) gm_load<4>(A.gate, b * A.gate_stride_t + h * A.gate_stride_h + d, A.gate_type, P.gvec, g);
+}
+
+// Four outputs of one head: o / l (0 where there was no key), times sigmoid(gate g).
+__device__ __forceinline__ void write_out(const Dec& P, int b, int h, int d, gm_f32x4 o, float l, const float (&g)[4]) {
+  const gm_paged_attn_args& A = P.a;
+  float v[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     v[e] = o[e] / l;
@@ -114,15 +121,22 @@ __device__ __forceinline__ void planes(const float (&v)[8], gm_u32x4 (&pl)[NP]) 
   }
 }
 
+// Blocks that a CU holds, one of a block's waves on each SIMD.  One more or less than this:
+// fp32 queries at 64 x 4,000 positions of 2 x 256 113 us (one: 128), 16 bits at 4 x 131,071
+// of 8 x 128 375 (two: 421), fp32 there with 4 heads 197 (two: 205), 32 x 8,000 of 8 x 64
+// 104 (three: 108).
+constexpr int per_cu(int Dh) { return Dh == 256 ? 2 : Dh == 128 ? 3 : 4; }
+
 template <int Dh, int QT, int NP>
-__global__ void __launch_bounds__(256, 2) k_paged_attn(Dec P) {
+__global__ void __launch_bounds__(256, per_cu(Dh)) k_paged_attn(Dec P) {
   using T = GmT16<QT>;
+  constexpr bool QLDS = NP > 1 || Dh == 256;        // queries in LDS: registers would spill
   constexpr int NC = Dh / 32;                       // MFMAs of a 16-key tile
   constexpr int VD = Dh < 128 ? 4 : 8;              // dims of a V row in a lane
   constexpr int DG = Dh / (16 * VD);                // V loads a row
   constexpr int LDO = Dh + 4;                       // floats between two heads' outputs in LDS
   constexpr float kShift = QT == GM_QTYPE_F16 ? 15.f : 0.f;        // p in f16: no subnormals to speak of
-  constexpr int QB = NP > 1 ? NP * NC * 1024 : 0, OB = 4 * 16 * LDO * 4;
+  constexpr int QB = QLDS ? NP * NC * 1024 : 0, OB = 4 * 16 * LDO * 4;
   __shared__ __attribute__((aligned(16))) char buf[QB > OB ? QB : OB];
   __shared__ float mls[4][16][2];
   __shared__ float qsc[16];
@@ -138,7 +152,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(Dec P) {
     for (int b = threadIdx.x / 64; b < A.n_seq; b += 4)
       if (pre[b] == pre[b + 1])
         for (int u = lane; u < nh * (Dh / 4); u += 64)
-          write_out(P, b, h0 + u / (Dh / 4), 4 * (u % (Dh / 4)), gm_f32x4{0.f, 0.f, 0.f, 0.f}, 0.f);
+          write_out(P, b, h0 + u / (Dh / 4), 4 * (u % (Dh / 4)), gm_f32x4{0.f, 0.f, 0.f, 0.f}, 0.f, {});
   }
   const int nb = min(P.nblk, R);                    // blocks that have a round, all of them
   if (i >= nb) return;
@@ -161,7 +175,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(Dec P) {
     if (s0 >= s1) continue;                         // a sequence without a key
     // ---- the queries: head n of the lane (those past nh repeat the last)
     const int64_t qrow = b * A.q_stride_t + (int64_t)(h0 + min(n, nh - 1)) * A.q_stride_h;
-    gm_u32x4 qf[NP > 1 ? 1 : NC];
+    gm_u32x4 qf[NP > 1 ? 1 : NC];                   // with QLDS on its way there
     float qs = A.scale;
     if constexpr (NP == 1) {
 #pragma unroll
@@ -173,7 +187,10 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(Dec P) {
 #pragma unroll
           for (int d = 0; d < 4; ++d) qf[c][d] = (uint32_t)q[2 * d] | (uint32_t)q[2 * d + 1] << 16;
         }
+        if constexpr (QLDS)
+          if (c % 4 == wave) *reinterpret_cast<gm_u32x4*>(buf + (c * 64 + lane) * 16) = qf[c];
       }
+      if constexpr (QLDS) __syncthreads();
     } else {
       // wave w stages heads 4 w .. 4 w + 3, 16 lanes a head
       const int hr = 4 * wave + g;
@@ -263,12 +280,17 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(Dec P) {
       if (r + 4 < s1) next = row_of(r + 4);
       // ---- scores
       gm_f32x4 s[2];
+      int q0 = lane * 16;                            // of the queries in LDS, unknown to the compiler, which
+      asm("" : "+v"(q0));                            // would else keep them all in registers over the rounds
       if constexpr (NP == 1) {
+        s[0] = s[1] = gm_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          s[t] = gm_f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int c = 0; c < NC; ++c) {
+          gm_u32x4 q;
+          if constexpr (QLDS) q = *reinterpret_cast<const gm_u32x4*>(buf + c * 1024 + q0);
+          else q = qf[c];
 #pragma unroll
-          for (int c = 0; c < NC; ++c) s[t] = T::mfma16(kf[t][c], qf[c], s[t]);
+          for (int t = 0; t < 2; ++t) s[t] = T::mfma16(kf[t][c], q, s[t]);
         }
       } else {
         gm_f32x4 odd[2];
@@ -278,7 +300,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(Dec P) {
         for (int p = NP - 1; p >= 0; --p)
 #pragma unroll
           for (int c = 0; c < NC; ++c) {
-            const gm_u32x4 q = *reinterpret_cast<const gm_u32x4*>(buf + ((p * NC + c) * 64 + lane) * 16);
+            const gm_u32x4 q = *reinterpret_cast<const gm_u32x4*>(buf + (p * NC + c) * 1024 + q0);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
               if (c & 1) odd[t] = T::mfma16(kf[t][c], q, odd[t]);
@@ -383,7 +405,9 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(Dec P) {
         lh = fmaf(mls[w][h][1], mw == kNegInf ? 0.f : exp2f((mw - Mh) * kLog2e), lh);
       }
       if (whole) {
-        write_out(P, b, h0 + h, d, o, lh);
+        float gt[4];
+        load_gate(P, b, h0 + h, d, gt);
+        write_out(P, b, h0 + h, d, o, lh, gt);
       } else {
         *reinterpret_cast<gm_f32x4*>(P.part + (slot + h) * Dh + d) = o;
         if (d == 0) {
@@ -398,19 +422,22 @@ __global__ void __launch_bounds__(256, 2) k_paged_attn(Dec P) {
 }
 
 // The parts of sequence b, head h (block b n_head + h), where it lies in more than
-// one block of k_paged_attn: out = sum_p o_p e^(m_p - M) / sum_p l_p e^(m_p - M).
-template <int Dh>
-__global__ void __launch_bounds__(512) k_paged_join(Dec P) {
-  constexpr int TP = Dh / 4, NGR = 512 / TP;
-  __shared__ int64_t red[8][2];
-  __shared__ float fred[8];
+// one block of k_paged_attn: out = sum_p o_p e^(m_p - M) / sum_p l_p e^(m_p - M).  Bound by
+// latency (lengths, maxima, parts): 7 us for 126 parts of 16 heads, 8 us for 1,024 blocks
+// of a few parts.  512 threads where there are fewer blocks than CUs (one sequence of 4,001:
+// 17.5 us in all, 18.5 with 256), else 256 (256 sequences of 32 heads: 204 and 219).
+template <int Dh, int NT>
+__global__ void __launch_bounds__(NT) k_paged_join(Dec P) {
+  constexpr int TP = Dh / 4, NGR = NT / TP;
+  __shared__ int64_t red[NT / 64][2];
+  __shared__ float fred[NT / 64];
   __shared__ __attribute__((aligned(16))) float os[NGR][Dh];
   extern __shared__ float wt[];                      // [nblk]
   const gm_paged_attn_args& A = P.a;
   const int b = blockIdx.x / A.n_head, h = blockIdx.x % A.n_head, tid = threadIdx.x;
   const int wave = tid >> 6, lane = tid & 63;
   int64_t before = 0, all = 0;
-  for (int j = tid; j < A.n_seq; j += 512) {
+  for (int j = tid; j < A.n_seq; j += NT) {
     const int c = (seq_len(P, j) + kRound - 1) / kRound;
     all += c;
     before += j < b ? c : 0;
@@ -423,7 +450,7 @@ __global__ void __launch_bounds__(512) k_paged_join(Dec P) {
   }
   __syncthreads();
   before = all = 0;
-  for (int w = 0; w < 8; ++w) {
+  for (int w = 0; w < NT / 64; ++w) {
     before += red[w][0];
     all += red[w][1];
   }
@@ -437,8 +464,11 @@ __global__ void __launch_bounds__(512) k_paged_join(Dec P) {
   auto slot = [&](int p) {
     return ((int64_t)(2 * (i0 + p) + (p == 0 ? 1 : 0)) * (A.n_head_kv * P.NG) + gy) * P.RG + hr;
   };
+  const int grp = tid / TP, d = 4 * (tid % TP);
+  float gt[4];                                       // loaded before the waits
+  load_gate(P, b, h, d, gt);
   float M = kNegInf;
-  for (int p = tid; p < np; p += 512) {
+  for (int p = tid; p < np; p += NT) {
     const float v = P.ml[2 * slot(p)];
     wt[p] = v;
     M = fmaxf(M, v);
@@ -447,14 +477,13 @@ __global__ void __launch_bounds__(512) k_paged_join(Dec P) {
   for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
   if (lane == 0) fred[wave] = M;
   __syncthreads();
-  for (int w = 0; w < 8; ++w) M = fmaxf(M, fred[w]);
+  for (int w = 0; w < NT / 64; ++w) M = fmaxf(M, fred[w]);
   __syncthreads();
-  for (int p = tid; p < np; p += 512) {
+  for (int p = tid; p < np; p += NT) {
     const float v = wt[p];
     wt[p] = v == kNegInf ? 0.f : exp2f((v - M) * kLog2e);
   }
   __syncthreads();
-  const int grp = tid / TP, d = 4 * (tid % TP);
   gm_f32x4 o = {0.f, 0.f, 0.f, 0.f};
   float l = 0.f;
 #pragma unroll 4
@@ -475,11 +504,10 @@ __global__ void __launch_bounds__(512) k_paged_join(Dec P) {
     o += *reinterpret_cast<const gm_f32x4*>(&os[q][d]);
     l += ls[q];
   }
-  write_out(P, b, h, d, o, l);
+  write_out(P, b, h, d, o, l, gt);
 }
 
-// Two blocks of four waves a CU hold every round that is in flight; more blocks
-// would only leave more parts to join.
+// As many blocks as the CUs hold at once; more would only leave more parts to join.
 Dec plan(const gm_paged_attn_args* a) {
   Dec P{};
   P.a = *a;
@@ -490,7 +518,8 @@ Dec plan(const gm_paged_attn_args* a) {
   P.cap = (int)(cap < 0x7fffff00 ? cap : 0x7fffff00);
   const int64_t rounds = (int64_t)a->n_seq * ((P.cap + kRound - 1) / kRound);
   const int ny = a->n_head_kv * P.NG;
-  const int64_t most = ny < 512 ? 512 / ny : 1;
+  const int held = 256 * per_cu(a->head_dim);
+  const int64_t most = ny < held ? held / ny : 1;
   P.nblk = (int)(rounds < 1 ? 1 : rounds < most ? rounds : most);
   return P;
 }
@@ -505,7 +534,9 @@ int launch(const Dec& P, hipStream_t s) {
   k_paged_attn<Dh, QT, NP><<<dim3(P.nblk, P.a.n_head_kv * P.NG), 256, lds, s>>>(P);
   GM_TRY(hipGetLastError());
   if (P.nblk == 1) return GM_OK;
-  k_paged_join<Dh><<<P.a.n_seq * P.a.n_head, 512, (size_t)P.nblk * 4, s>>>(P);
+  const int heads = P.a.n_seq * P.a.n_head;
+  if (heads < 256) k_paged_join<Dh, 512><<<heads, 512, (size_t)P.nblk * 4, s>>>(P);
+  else k_paged_join<Dh, 256><<<heads, 256, (size_t)P.nblk * 4, s>>>(P);
   GM_TRY(hipGetLastError());
   return GM_OK;
 }
