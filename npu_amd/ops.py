@@ -200,13 +200,15 @@ def _elem(t: torch.Tensor, name: str, among=_ELEM) -> int:
     return _ELEM[t.dtype]
 
 
-def _rows(t: torch.Tensor, name: str, shape) -> torch.Tensor:
-    """t, of the given shape ([.., heads, head_dim]) and with contiguous rows of head_dim."""
+def _rows(t: torch.Tensor, name: str, shape) -> tuple[int, int]:
+    """The strides of t's tokens and heads; t must have the given shape [T, heads, head_dim]
+    (or be pages) and contiguous rows of head_dim."""
     if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-    if t.stride(-1) != 1:
+    st = t.stride()
+    if st[-1] != 1:
         raise ValueError(f"{name}: the last dim must be contiguous")
-    return t
+    return st[:2]
 
 
 def _ints(t: torch.Tensor, name: str, shape) -> torch.Tensor:
@@ -232,44 +234,60 @@ def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor):
     return (ct, *k_pages.shape)
 
 
-def _out(out: torch.Tensor | None, shape, dtype: torch.dtype, like: torch.Tensor) -> torch.Tensor:
+def _out(out: torch.Tensor | None, shape, dtype: torch.dtype, like: torch.Tensor, *inputs) -> torch.Tensor:
+    """``out``, or a new tensor; one that is given must not overlap ``like`` or ``inputs``, which
+    blocks read while others write."""
     if out is None:
         return torch.empty(shape, dtype=dtype, device=like.device)
     if out.shape != shape or out.dtype != dtype or not out.is_contiguous():
         raise ValueError(f"out must be contiguous {list(shape)} {dtype}, got {list(out.shape)} {out.dtype}")
+    lo, hi = _span(out)
+    for t in (like, *inputs):
+        if t is not None:
+            a, b = _span(t)
+            if a < hi and lo < b:
+                raise ValueError("out overlaps an input")
     return out
 
 
-def _one_device(first: torch.Tensor, *others: torch.Tensor | None) -> torch.device:
-    dev = first.device
-    if dev.type != "cuda":
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """The addresses between t's first byte and its last."""
+    if t.numel() == 0:
+        return 0, 0
+    p = t.data_ptr()
+    return p, p + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _one_device(first: torch.Tensor, *others: torch.Tensor | None) -> int:
+    dev = first.get_device()
+    if dev < 0:
         raise ValueError("tensors must be on the GPU")
     for t in others:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
     return dev
 
 
-def _ptr(t: torch.Tensor | None) -> int | None:
-    return None if t is None else t.data_ptr()
+def _ptr(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
-def _enqueue(dev: torch.device, name: str, args, ws_bytes=None) -> None:
-    """Call the entry point ``name`` on ``dev``'s current stream; with ``ws_bytes`` (the name of
-    its size query) it gets a workspace of its own."""
-    if dev.index != torch.cuda.current_device():
+def _enqueue(dev: int, name: str, args, ws_bytes=None) -> None:
+    """Call the entry point ``name`` on the current stream of device ``dev``; with ``ws_bytes``
+    (the name of its size query) it gets a workspace of its own."""
+    if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
             return _enqueue(dev, name, args, ws_bytes)
     lib = L.lib()
-    ref = ctypes.byref(args)
+    stream = torch.cuda.current_stream(dev).cuda_stream
     if ws_bytes is None:
-        rc = getattr(lib, name)(ref, L.stream_ptr())
+        rc = getattr(lib, name)(args, stream)
     else:
-        n = getattr(lib, ws_bytes)(ref)
+        n = getattr(lib, ws_bytes)(args)
         if n == 0:
             L.check(L.GM_EINVAL, name)
         ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        rc = getattr(lib, name)(ref, ws.data_ptr(), n, L.stream_ptr())
+        rc = getattr(lib, name)(args, ws.data_ptr(), n, stream)
     L.check(rc, name)
 
 
@@ -295,9 +313,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     if q.dim() != 3:
         raise ValueError(f"q must be [T, n_head, head_dim], got {list(q.shape)}")
     T, hq, _ = q.shape
-    _rows(q, "q", (T, hq, dh))
-    _rows(k, "k", (T, hkv, dh))
-    _rows(v, "v", (T, hkv, dh))
+    strides = *_rows(q, "q", (T, hq, dh)), *_rows(k, "k", (T, hkv, dh)), *_rows(v, "v", (T, hkv, dh))
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError("q, k and v must have one type")
     n_axes = positions.shape[0] if positions.dim() == 2 else 1
@@ -314,12 +330,12 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     if not (positions.is_contiguous() and slots.is_contiguous() and (axis is None or axis.is_contiguous())):
         raise ValueError("positions, slots and axis must be contiguous")
     dev = _one_device(q, k, v, positions, inv_freq, k_pages, v_pages, slots, axis, q_norm, k_norm, out)
-    out = _out(out, (T, hq, dh), out_dtype or (k_pages.dtype if out is None else out.dtype), q)
-    a = L.GmRopeAppendArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(),
-                           _ptr(axis), _ptr(q_norm), _ptr(k_norm), out.data_ptr(), k_pages.data_ptr(),
-                           v_pages.data_ptr(), slots.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1),
-                           v.stride(0), v.stride(1), n_pages * page, eps, T, n_axes, hq, hkv, dh, 2 * half, in_type,
-                           _elem(out, "out"), ct)
+    out = _out(out, (T, hq, dh), out_dtype or (k_pages.dtype if out is None else out.dtype), q, k, v, k_pages, v_pages,
+               positions, slots)
+    a = L.filled(L.GmRopeAppendArgs, q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr(),
+                 inv_freq.data_ptr(), _ptr(axis), _ptr(q_norm), _ptr(k_norm), out.data_ptr(), k_pages.data_ptr(),
+                 v_pages.data_ptr(), slots.data_ptr(), *strides, n_pages * page, eps, T, n_axes, hq, hkv, dh, 2 * half,
+                 in_type, _elem(out, "out"), ct)
     _enqueue(dev, "gm_rope_append", a)
     return out
 
@@ -339,7 +355,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if q.dim() != 3:
         raise ValueError(f"q must be [n_seq, n_head, head_dim], got {list(q.shape)}")
     B, hq, _ = q.shape
-    _rows(q, "q", (B, hq, dh))
+    qs = _rows(q, "q", (B, hq, dh))
     _ints(lengths, "lengths", (B,))
     if block_table.dim() != 2:
         raise ValueError(f"block_table must be [n_seq, width], got {list(block_table.shape)}")
@@ -347,19 +363,17 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     _ints(block_table, "block_table", (B, width))
     if (width > 1 and block_table.stride(1) != 1) or not lengths.is_contiguous():
         raise ValueError("lengths and the rows of block_table must be contiguous")
-    gt = gs0 = gs1 = 0
+    gt, gs = 0, (0, 0)
     if gate is not None:
         gt = _elem(gate, "gate")
-        _rows(gate, "gate", (B, hq, dh))
-        gs0, gs1 = gate.stride(0), gate.stride(1)
+        gs = _rows(gate, "gate", (B, hq, dh))
     dev = _one_device(q, k_pages, v_pages, block_table, lengths, gate, out)
-    out = _out(out, (B, hq, dh), q.dtype, q)
+    out = _out(out, (B, hq, dh), q.dtype, q, k_pages, v_pages, block_table, lengths, gate)
     if B == 0:
         return out
-    a = L.GmPagedAttnArgs(q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(),
-                          lengths.data_ptr(), _ptr(gate), out.data_ptr(), q.stride(0), q.stride(1), gs0, gs1,
-                          block_table.stride(0) if B > 1 else width, dh ** -0.5 if scale is None else scale, B, hq,
-                          hkv, dh, n_pages, page, width, qt, ct, gt)
+    a = L.filled(L.GmPagedAttnArgs, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(),
+                 lengths.data_ptr(), _ptr(gate), out.data_ptr(), *qs, *gs, block_table.stride(0) if B > 1 else width,
+                 dh ** -0.5 if scale is None else scale, B, hq, hkv, dh, n_pages, page, width, qt, ct, gt)
     _enqueue(dev, "gm_paged_attention", a, "gm_paged_attention_workspace_bytes")
     return out
 
@@ -388,7 +402,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     if cu_q.dim() != 1 or n_seq < 0:
         raise ValueError("cu_q must be [n_seq + 1]")
     _ints(cu_q, "cu_q", (n_seq + 1,))
-    _rows(q, "q", (n_q, hq, dh))
+    qs = _rows(q, "q", (n_q, hq, dh))
     n_k = n_pages = page = width = ts = 0
     if paged:
         _, n_pages, page, hkv, _ = _pages(k, v)
@@ -400,28 +414,25 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
         if (width > 1 and block_table.stride(1) != 1) or not lengths.is_contiguous():
             raise ValueError("lengths and the rows of block_table must be contiguous")
         ts = block_table.stride(0) if n_seq > 1 else width
-        ks0 = ks1 = vs0 = vs1 = 0
     else:
         n_k, hkv, _ = k.shape
         cu_k = cu_q if cu_k is None else _ints(cu_k, "cu_k", (n_seq + 1,))
-        ks0, ks1, vs0, vs1 = k.stride(0), k.stride(1), v.stride(0), v.stride(1)
     if k.shape[-1] != dh:
         raise ValueError(f"k has head_dim {k.shape[-1]}, q {dh}")
-    _rows(k, "k", k.shape)
-    _rows(v, "v", k.shape)
+    ks, vs = _rows(k, "k", k.shape), _rows(v, "v", k.shape)
+    if paged:
+        ks = vs = (0, 0)
     if not cu_q.is_contiguous() or (cu_k is not None and not cu_k.is_contiguous()):
         raise ValueError("cu_q and cu_k must be contiguous")
-    gt = gs0 = gs1 = 0
+    gt, gs = 0, (0, 0)
     if gate is not None:
         gt = _elem(gate, "gate")
-        _rows(gate, "gate", (n_q, hq, dh))
-        gs0, gs1 = gate.stride(0), gate.stride(1)
+        gs = _rows(gate, "gate", (n_q, hq, dh))
     dev = _one_device(q, k, v, cu_q, cu_k, block_table, lengths, gate, out)
-    out = _out(out, (n_q, hq, dh), q.dtype, q)
-    a = L.GmPromptAttnArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), _ptr(cu_k), _ptr(block_table),
-                           _ptr(lengths), _ptr(gate), out.data_ptr(), q.stride(0), q.stride(1), ks0, ks1, vs0, vs1,
-                           gs0, gs1, ts, dh ** -0.5 if scale is None else scale, n_q, n_k, n_seq, hq, hkv, dh,
-                           n_pages, page, width, qt, gt)
+    out = _out(out, (n_q, hq, dh), q.dtype, q, k, v, cu_q, cu_k, block_table, lengths, gate)
+    a = L.filled(L.GmPromptAttnArgs, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_q.data_ptr(), _ptr(cu_k),
+                 _ptr(block_table), _ptr(lengths), _ptr(gate), out.data_ptr(), *qs, *ks, *vs, *gs, ts,
+                 dh ** -0.5 if scale is None else scale, n_q, n_k, n_seq, hq, hkv, dh, n_pages, page, width, qt, gt)
     _enqueue(dev, "gm_prompt_attention", a)
     return out
 
@@ -457,10 +468,10 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature: float | torch.
             held.append(None)
             alone.append(none if val is None else val)
     dev = _one_device(logits, u, *held, out)
-    out = _out(out, (B,), torch.int64, logits)
+    out = _out(out, (B,), torch.int64, logits, u, *held)
     if B == 0:
         return out
-    a = L.GmSampleArgs(logits.data_ptr(), u.data_ptr(), *(_ptr(t) for t in held), out.data_ptr(),
-                       logits.stride(0) if B > 1 else V, *alone, B, V, lt)
+    a = L.filled(L.GmSampleArgs, logits.data_ptr(), u.data_ptr(), *(_ptr(t) for t in held), out.data_ptr(),
+                 logits.stride(0) if B > 1 else V, *alone, B, V, lt)
     _enqueue(dev, "gm_sample", a, "gm_sample_workspace_bytes")
     return out

@@ -698,3 +698,29 @@ def test_tensors_on_the_host_are_refused(gpu):
     x, u = torch.zeros(1, 8, device="cuda"), torch.zeros(1)
     with pytest.raises(ValueError, match="different devices"):
         ops.sample(x, u)
+
+
+def test_outputs_over_inputs_and_values_out_of_range_are_refused(gpu):
+    g = _g(41)
+    q = _randn(g, 2, 4, 64, dtype=BF)
+    k, v, table = _paged(g, [20, 9], 16, 2, 64, BF, poison=False)
+    n = torch.tensor([20, 9], dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.paged_attention(q, k, v, table, n, out=q)
+    rows = _randn(g, 3, 4, 128, dtype=BF)
+    cu = torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+    kv = _randn(g, 3, 2, 64, dtype=BF)
+    flat = rows.view(-1)[:3 * 4 * 64].view(3, 4, 64)
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.prompt_attention(rows[..., 64:], kv, kv, cu, out=flat)
+    out = torch.empty(3, 4, 64, dtype=BF, device="cuda")
+    assert ops.prompt_attention(rows[..., 64:], kv, kv, cu, out=out) is out
+    x, u = _randn(g, 2, 100), torch.rand(2, device="cuda")
+    for kw in (dict(top_k=2 ** 40), dict(top_k=2.5)):
+        with pytest.raises(ValueError, match="GmSampleArgs"):
+            ops.sample(x, u, **kw)
+    # past fp32's range is infinity, as in any fp32 tensor
+    assert ops.sample(x, u, temperature=1e300).tolist() == ops.sample(x, u, temperature=math.inf).tolist()
+    buf = torch.zeros(4, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError, match="overlaps"):
+        ops.sample(x, buf.view(torch.float32)[:2], out=buf[:2])
