@@ -414,11 +414,16 @@ __device__ __forceinline__ void hist_find(Shared& S, unsigned long long tlo, uns
 // with a low temperature ends far out: with all bins 1/128 wide, 64 rows with a 300th
 // value 33 temperatures away took 750 us instead of 50.
 __device__ __forceinline__ int dist_bin(float x, const Row& R) {
-  if (!(x > kNegInf)) return -1;
-  if (x == R.xmax) return 0;
   const float d = (R.xmax - x) * R.per_bin;
-  const float b = d < (float)kFine ? d : (float)kFine + (d - (float)kFine) * (1.f / 16);
-  return b < (float)(kBins - 1) ? (int)b : kBins - 1;
+  // the two slopes' lesser; NaN (an infinite maximum or reach) goes to the last bin
+  const float b = fminf(fminf(d, fmaf(d, 1.f / 16, (float)kFine * (15.f / 16))), (float)(kBins - 1));
+  const int bin = x == R.xmax ? 0 : (int)b;
+  return x > kNegInf ? bin : -1;
+}
+
+// The weight of x where dist_bin is not the last: no further than 272 temperatures.
+__device__ __forceinline__ double near_weight(float x, const Row& R, const double* tab) {
+  return fexp(x == R.xmax ? 0.0 : ((double)x - (double)R.xmax) * R.units, tab);
 }
 
 // A weight in fp32 as a multiple of 2^-32, rounded down.  The exponent's rounding is the
@@ -521,7 +526,7 @@ __device__ __forceinline__ Cut find_cut(const Smp& P, Shared& S, const float* gm
       const int b = dist_bin(v.x[j], R);
       if (b < 0 || b > hi) continue;
       if (b < lo) {
-        const double w = weight(v.x[j], R.xmax, R.units, S.tab);
+        const double w = near_weight(v.x[j], R, S.tab);
         sum += w;
         own += w >= minw ? w : 0.0;
       } else {
