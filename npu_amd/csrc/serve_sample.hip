@@ -26,8 +26,10 @@
 // rows the second kernel's chain of block-wide steps, for many flat rows its two passes.
 //
 // Measured, first and second kernel: one row of 248,320 fp32 with all filters 3 + 22 us;
-// 64 rows of 248,320 fp32 with mixed filters 20 (3.2 TB/s) + 31 us; 256 rows of 248,320 bf16 and their
-// nuclei of up to half the vocabulary 67 us (1.9 TB/s, beside its 64 M exponentials) + 232.
+// 64 rows of 248,320 fp32 with mixed filters 20 (3.2 TB/s) + 31 us; 256 rows of 248,320 bf16
+// and their nuclei 67 us (1.9 TB/s, beside its 64 M exponentials) + 200.  The 200 are those of
+// the few flat rows, each on one CU: 50 for the histogram, 80 for the pass in 64 bits, 50
+// instructions a value in both; rows of up to kCand candidates are done after 20 to 60.
 #include "kernels.h"
 #include "serving.h"
 
@@ -421,6 +423,18 @@ __device__ __forceinline__ int dist_bin(float x, const Row& R) {
   return x > kNegInf ? bin : -1;
 }
 
+// The least x whose bin is below `bin`, NaN for bin 0: two comparisons sort a value among
+// the bins' ends instead of its bin.
+__device__ __forceinline__ float bin_end(int bin, const Row& R) {
+  uint32_t no = key_of(kNegInf, 0), yes = key_of(R.xmax, 0);
+  while (yes - no > 1) {                                // 32 times at most
+    const uint32_t mid = no + (yes - no) / 2;
+    if (dist_bin(value_of(mid, 0), R) < bin) yes = mid;
+    else no = mid;
+  }
+  return bin > 0 ? value_of(yes, 0) : __builtin_nanf("");
+}
+
 // The weight of x where dist_bin is not the last: no further than 272 temperatures.
 __device__ __forceinline__ double near_weight(float x, const Row& R, const double* tab) {
   return fexp(x == R.xmax ? 0.0 : ((double)x - (double)R.xmax) * R.units, tab);
@@ -508,6 +522,8 @@ __device__ __forceinline__ Cut find_cut(const Smp& P, Shared& S, const float* gm
   }
   const int lo = S.lo, hi = min(max(S.hi, lo), limit);
   const int above_n = by_count ? (int)S.above : 0;
+  const float xa = bin_end(lo, R), xm = bin_end(hi + 1, R);      // above the interval x >= xa, with it x >= xm
+  const bool by_min = minw > 0.0;
   // the weight above the interval in 64 bits, and its members: how many, their least and
   // largest key, and themselves if they are few
   if (tid == 0) S.count = 0;
@@ -520,16 +536,21 @@ __device__ __forceinline__ Cut find_cut(const Smp& P, Shared& S, const float* gm
   uint32_t least = 0xffffffffu, most = 0u;
   each_group(P, gmax, R, hi, [&](int g, const Lane8& v) {
     double own = 0.0;
-    const bool room = *static_cast<volatile int*>(&S.count) <= kCand;
+    bool in = false;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int b = dist_bin(v.x[j], R);
-      if (b < 0 || b > hi) continue;
-      if (b < lo) {
-        const double w = near_weight(v.x[j], R, S.tab);
-        sum += w;
-        own += w >= minw ? w : 0.0;
-      } else {
+      // no branch: the eight exponentials overlap
+      const bool up = v.x[j] >= xa;
+      const double e = near_weight(up ? v.x[j] : R.xmax, R, S.tab), w = up ? e : 0.0;
+      if (by_min) sum += w;
+      own += by_min && w < minw ? 0.0 : w;
+      in |= v.x[j] >= xm && !up;
+    }
+    if (in) {
+      const bool room = *static_cast<volatile int*>(&S.count) <= kCand;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (!(v.x[j] >= xm) || v.x[j] >= xa) continue;
         const uint32_t key = key_of(v.x[j], R.low);
         least = min(least, key);
         most = max(most, key);
@@ -537,6 +558,7 @@ __device__ __forceinline__ Cut find_cut(const Smp& P, Shared& S, const float* gm
         if (at < kCand) S.cand[at] = (unsigned long long)~key << 32 | (uint32_t)v.at(j);
       }
     }
+    if (!by_min) sum += own;
     own = wave_sum(own);
     if (lane == 0) gs[g] = own;
   });
@@ -591,8 +613,7 @@ __device__ __forceinline__ Cut find_cut(const Smp& P, Shared& S, const float* gm
     each_group(P, gmax, R, hi, [&](int, const Lane8& v) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int b = dist_bin(v.x[j], R);
-        if (b < lo || b > hi) continue;                 // lo >= 0
+        if (!(v.x[j] >= xm) || v.x[j] >= xa) continue;
         const uint32_t d = most - key_of(v.x[j], R.low);
         if ((d & known) != gap) continue;
         const unsigned long long one =
@@ -616,8 +637,7 @@ __device__ __forceinline__ Cut find_cut(const Smp& P, Shared& S, const float* gm
     int e = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int b = dist_bin(v.x[j], R);
-      if (b < lo || b > hi) continue;
+      if (!(v.x[j] >= xm) || v.x[j] >= xa) continue;
       const uint32_t key = key_of(v.x[j], R.low);
       if (key > c.key) {
         const double w = weight(v.x[j], R.xmax, R.units, S.tab);
