@@ -406,13 +406,14 @@ int gm_moe_forward_noalloc(const gm_moe_layer* L, const float* x, float* y, int 
  * each sequence in order.  A page number outside [0, n_pages) holds no keys: its
  * positions are masked.  head_dim is 64, 128 or 256; n_head a multiple of
  * n_head_kv, scale positive.  Every length, offset and table is read on the device
- * only.
+ * only, and lengths past 2^31 - 256 count as that.
  */
 
 /*
  * q_out = rot(rmsnorm(q) q_norm), and rot(rmsnorm(k) k_norm) and v to the
  * cache's row slots[t] (page number times page_size plus the row in the page; one
- * outside [0, n_rows) writes nothing; a slot given twice keeps either row).
+ * outside [0, n_rows) writes nothing; of a slot given twice each 16 bytes are one
+ * of the two tokens').
  * rot turns the pairs (i, i + rope_dim / 2) by positions[axis[i]][t] * inv_freq[i]
  * radians, formed in 64 bits; dims from rope_dim on are not turned.  rope_dim is
  * even and at most head_dim.  The norms are left out where q_norm / k_norm is NULL.

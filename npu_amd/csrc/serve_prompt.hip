@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(64 * NW, WPS) k_prompt_attn(Pmt P) {
   const int q0 = cuq(b), nq = max(cuq(b + 1) - q0, 0);
   int k0 = 0, nk;
   if constexpr (PAGED) {
-    const int64_t cap = (int64_t)A.table_width * A.page_size;
+    const int64_t cap = min((int64_t)A.table_width * A.page_size, (int64_t)0x7fffff00);   // room to round up
     nk = max(A.lengths[b], 0);
     if (nk > cap) nk = (int)cap;
   } else {

@@ -215,6 +215,27 @@ def test_paged_attention_many_sequences(gpu, dtype, ct):
     _check_decode(out, q, k, v, table, lengths, 16, 0.2, None, dtype, ct)
 
 
+@pytest.mark.parametrize("dh", [64, 256])
+def test_paged_attention_the_most_sequences(gpu, dh):
+    """8,192 of them, the largest tables of rounds in LDS; a page of its own for each, shared by
+    the first and the last."""
+    g = _g(6)
+    B = 8192
+    lengths = torch.randint(0, 4, (B,), generator=g, device="cuda", dtype=torch.int32)
+    lengths[0] = lengths[-1] = 3
+    k, v = (_randn(g, B, 4, 1, dh, dtype=BF) for _ in range(2))
+    table = torch.arange(B, dtype=torch.int32, device="cuda")[:, None].clone()
+    table[-1] = 0
+    q = _randn(g, B, 2, dh, dtype=BF)
+    out = ops.paged_attention(q, k, v, table, lengths)
+    kk, vv = k[table[:, 0].long(), :, 0].double(), v[table[:, 0].long(), :, 0].double()
+    x = (q.double()[:, :, None] * kk[:, None]).sum(-1) * dh ** -0.5
+    dead = torch.arange(4, device="cuda") >= lengths[:, None]
+    p = torch.softmax(x.masked_fill(dead[:, None], -math.inf), -1).nan_to_num(0.0)
+    want, absv = ((p[..., None] * f[:, None]).sum(2) for f in (vv, vv.abs()))
+    _close(out, want, _tol(want, absv, vv, BF, BF))
+
+
 def test_paged_attention_one_long_sequence(gpu):
     """70,001 positions over all blocks, scores far apart, q rows at odd elements."""
     g = _g(6)
@@ -554,6 +575,21 @@ def test_sample_one_row_each(gpu, V, dtype):
     tb, kb, pb, mb = FILTERS[b]
     one = ops.sample(x[b:b + 1].contiguous(), u[b:b + 1].contiguous(), temperature=tb, top_k=kb, top_p=pb, min_p=mb)
     assert one.tolist() == [want[b]]
+
+
+@pytest.mark.parametrize("dtype", [F32, HF])
+def test_sample_the_largest_vocabulary(gpu, dtype):
+    g = _g(2)
+    V = 2 ** 21
+    rows = [(0.7, 50, 0.9, 0.0), (1.0, 0, 0.7, 0.0), (1.0, 5000, 1.0, 0.0), (1.0, 0, 1.0, 0.0), (0.0, 0, 1.0, 0.0)]
+    x = _randn(g, len(rows), V, scale=1.5).to(dtype)
+    u = torch.rand(len(rows), generator=g, device="cuda")
+    t, k, p, mp = (torch.tensor(c, dtype=d, device="cuda") for c, d in zip(zip(*rows), (F32, torch.int32, F32, F32)))
+    got = ops.sample(x, u, temperature=t, top_k=k, top_p=p, min_p=mp)
+    assert got.tolist() == [_sample_ref(x[b], float(u[b]), *(_f32(f) if i != 1 else f for i, f in enumerate(rows[b])))
+                            for b in range(len(rows))]
+    with pytest.raises(ValueError, match="vocab"):
+        ops.sample(torch.empty(1, V + 1, dtype=dtype, device="cuda"), u[:1])
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
