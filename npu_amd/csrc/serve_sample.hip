@@ -960,7 +960,11 @@ int gm_sample_run(const gm_sample_args* a, uint8_t* ws, hipStream_t s) {
   else k_sample_groups<1><<<dim3((P.ng + 3) / 4, a->n_row), 256, 0, s>>>(P);
   GM_TRY(hipGetLastError());
   const size_t lds = sizeof(Shared) + (size_t)P.ng * 20;
-  if (int rc = gm_set_smem(k_sample_pick, lds)) return rc;
+  // one limit for every vocabulary: two threads' calls must not lower it for each other
+  constexpr size_t most = sizeof(Shared) + ((1 << 21) / kGroup) * 20;
+  static_assert(most <= 160 * 1024);
+  if (lds > 65536)
+    if (int rc = gm_set_smem(k_sample_pick, most)) return rc;
   k_sample_pick<<<a->n_row, kThreads, lds, s>>>(P);
   GM_TRY(hipGetLastError());
   return GM_OK;

@@ -191,13 +191,15 @@ def moe_chain_fused(layers, T: int) -> bool:
 
 
 # ------------------------------------------------------------ serving a batch
-_ELEM = {torch.float32: L.GM_QTYPE_F32, torch.float16: L.GM_QTYPE_F16, torch.bfloat16: L.GM_QTYPE_BF16}
+_T16 = {torch.float16: L.GM_QTYPE_F16, torch.bfloat16: L.GM_QTYPE_BF16}
+_ELEM = {torch.float32: L.GM_QTYPE_F32, **_T16}
 
 
 def _elem(t: torch.Tensor, name: str, among=_ELEM) -> int:
-    if t.dtype not in among:
+    qtype = among.get(t.dtype)
+    if qtype is None:
         raise TypeError(f"{name} must be {' or '.join(str(d) for d in among)}, got {t.dtype}")
-    return _ELEM[t.dtype]
+    return qtype
 
 
 def _rows(t: torch.Tensor, name: str, shape) -> tuple[int, int]:
@@ -217,9 +219,6 @@ def _ints(t: torch.Tensor, name: str, shape) -> torch.Tensor:
     if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
     return t
-
-
-_T16 = (torch.bfloat16, torch.float16)
 
 
 def _pages(k_pages: torch.Tensor, v_pages: torch.Tensor):
@@ -272,6 +271,11 @@ def _ptr(t: torch.Tensor | None) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+# the number alone: rope_append of 8 tokens takes 12.6 us of host time, 14.2 with the stream as an object
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
 def _enqueue(dev: int, name: str, args, ws_bytes=None) -> None:
     """Call the entry point ``name`` on the current stream of device ``dev``; with ``ws_bytes``
     (the name of its size query) it gets a workspace of its own."""
@@ -279,7 +283,7 @@ def _enqueue(dev: int, name: str, args, ws_bytes=None) -> None:
         with torch.cuda.device(dev):
             return _enqueue(dev, name, args, ws_bytes)
     lib = L.lib()
-    stream = torch.cuda.current_stream(dev).cuda_stream
+    stream = _stream_of(dev)
     if ws_bytes is None:
         rc = getattr(lib, name)(args, stream)
     else:
