@@ -451,6 +451,8 @@ int gm_rope_append(const gm_rope_append_args* a, void* stream);
  * as that.  q and out are F32 (any cache type) or the cache's type.  n_seq is at
  * most 8192.  Work is split over the lengths and joined by a second launch;
  * partial results are in the workspace, and no result depends on what else runs.
+ * What a mask leaves out may be anything; where a sequence does see a K or V that is
+ * not finite, the outputs it reaches are infinite or NaN.
  */
 typedef struct gm_paged_attn_args {
   const void* q;             /* [n_seq][n_head][head_dim] in q_type */

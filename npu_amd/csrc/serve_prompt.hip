@@ -1,6 +1,6 @@
 // Causal attention over packed prompts (gm_prompt_attention), keys packed or in
-// the cache's pages: out = softmax(scale q K^T + mask) V in one pass over the keys
-// with a running maximum m and sum l per row.
+// the cache's pages: out = softmax(scale q K^T + mask) V in one pass over the keys,
+// with a row's exponentials taken relative to a fixed reference.
 //
 // Rows: a kv head's rows of one sequence are its tokens x G = n_head / n_head_kv
 // heads, head fastest, so that a block's rows share nearly all their keys.  A wave has
@@ -29,6 +29,12 @@
 // A masked key has p = 0, and 0 times a V value that is not finite would be NaN: such
 // values are cleared in the tiles with a mask, and added at the end to the rows that
 // see them.
+//
+// Bound: MFMA, with the exponentials beside them; for short prompts the latency of a
+// block's first loads and its epilogue.  Measured: 16,000 tokens of 16 heads of 256 on 2,
+// bf16, 2.32 ms (900 TFLOP/s of the 1,110 of a large product); 8,192 tokens in 11 prompts,
+// 32 heads of 128 on 8, fp16, 136 us (675); 301 tokens in 5, 16 of 256, 30 us.  With a
+// running maximum and the rescaling the first took 15.6 ms, its registers spilled.
 #include "kernels.h"
 #include "serving.h"
 
@@ -539,7 +545,7 @@ int launch_size(const Pmt& P, hipStream_t s) {
   if constexpr (Dh == 256) {
     // heads of 256 take 128 registers for o and 64 for q: two waves a SIMD hold that only
     // with 10 of the 16 pieces of q in LDS, which one block of 8 waves a CU has room for
-    // (16,000 tokens: 2.19 ms; all in registers and spilled 2.95, one wave a SIMD 3.3).
+    // (16,000 tokens: 2.3 ms; all in registers and spilled 2.95, one wave a SIMD 3.3).
     // Where such blocks would leave CUs idle, 4 waves with everything in registers
     // (301 tokens: 29.7 us against 33.5)
     if ((int64_t)P.a.n_q * P.a.n_head / 256 < 256) return launch<Dh, QT, PAGED, 4, 32, 0, 4, 4, 1>(P, s);

@@ -760,3 +760,56 @@ def test_outputs_over_inputs_and_values_out_of_range_are_refused(gpu):
     buf = torch.zeros(4, dtype=torch.int64, device="cuda")
     with pytest.raises(ValueError, match="overlaps"):
         ops.sample(x, buf.view(torch.float32)[:2], out=buf[:2])
+
+
+def test_calls_on_two_streams_at_once(gpu):
+    """Every operator on two streams in turn, with nothing between: each call's result is the
+    one it gives alone."""
+    g = _g(51)
+    x, u = _logits(g, 40, 50_001, BF), torch.rand(40, generator=g, device="cuda")
+    q, k, v = (_randn(g, 900, h, 128, dtype=HF) for h in (8, 2, 2))
+    cu = torch.tensor([0, 200, 201, 900], dtype=torch.int32, device="cuda")
+    kp, vp, table = _paged(g, [700, 3, 90], 16, 2, 128, HF, poison=False)
+    n = torch.tensor([700, 3, 90], dtype=torch.int32, device="cuda")
+    calls = (lambda: ops.sample(x, u, temperature=1.1, top_p=0.9), lambda: ops.sample(x, u, top_k=700, min_p=0.01),
+             lambda: ops.prompt_attention(q, k, v, cu), lambda: ops.paged_attention(q[:3], kp, vp, table, n))
+    want = [f() for f in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for i in range(6):
+        for j, f in enumerate(calls):
+            with torch.cuda.stream(streams[(i + j) % 2]):
+                got.append((j, f()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[j]) for j, o in got)
+
+
+@pytest.mark.parametrize("dtype,ct", TYPES)
+def test_paged_attention_values_that_are_not_finite(gpu, dtype, ct):
+    """An infinite or NaN V that a sequence sees shows in its dim, and nowhere else."""
+    g = _g(52)
+    k, v, table = _paged(g, [300, 300], 16, 2, 128, ct, poison=False)
+    table[1] = table[0]
+    q = _randn(g, 2, 8, 128, dtype=dtype)
+    n = torch.tensor([300, 40], dtype=torch.int32, device="cuda")
+    clean = ops.paged_attention(q, k, v, table, n)
+    page, row = int(table[0, 6]), 4                      # position 100: of the first sequence alone
+    v[page, row, 0, 5], v[page, row, 1, 77] = float("inf"), float("nan")
+    out = ops.paged_attention(q, k, v, table, n)
+    assert torch.equal(out[1], clean[1])
+    assert not torch.isfinite(out[0, :4, 5]).any() and bool(out[0, 4:, 77].isnan().all())
+    out[0, :4, 5], out[0, 4:, 77] = clean[0, :4, 5], clean[0, 4:, 77]
+    assert torch.equal(out, clean)
+
+
+def test_prompt_attention_heads_that_are_expanded(gpu):
+    g = _g(53)
+    q, k, v = (_randn(g, 150, h, 64, dtype=BF) for h in (6, 1, 1))
+    cu = torch.tensor([0, 31, 150], dtype=torch.int32, device="cuda")
+    want = ops.prompt_attention(q, k, v, cu)
+    got = ops.prompt_attention(q, k.expand(-1, 3, -1), v.expand(-1, 3, -1), cu)
+    for b, (i, j) in enumerate(((0, 31), (31, 150))):
+        ref, absv = _attend_ref(q[i:j], k[i:j], v[i:j], 64 ** -0.5, torch.arange(j - i, device="cuda"))
+        for o in (want, got):
+            _close(o[i:j], ref, _tol(ref, absv, v, BF, BF))
