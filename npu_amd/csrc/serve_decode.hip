@@ -332,13 +332,17 @@ __global__ void __launch_bounds__(256, per_cu(Dh)) k_paged_attn(Dec P) {
       m = mn;
       float sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p[j] = exp2f(fmaf(p[j] - mr, kLog2e, kShift));
-        sum += p[j];
-      }
-      l = fmaf(l, al, sum);
+      for (int j = 0; j < 8; ++j) p[j] = exp2f(fmaf(p[j] - mr, kLog2e, kShift));
       gm_u32x4 pp[NP];
       planes<QT, NP>(p, pp);
+      if constexpr (NP == 1) {                       // as rounded: few keys then divide the rounding out
+#pragma unroll
+        for (int w = 0; w < 4; ++w) sum = T::add(pp[0][w], sum);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += p[j];
+      }
+      l = fmaf(l, al, sum);
       const uint32_t flip = NP > 1 && (r & 4) ? 0x80008000u : 0u;
       const float sgn = NP > 1 && (r & 4) ? -1.f : 1.f;
       if constexpr (NP > 1) {

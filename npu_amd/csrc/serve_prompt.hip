@@ -404,8 +404,8 @@ __global__ void __launch_bounds__(64 * NW, WPS) k_prompt_attn(Pmt P) {
           if (w < NS * 8) {
             const float a = __builtin_amdgcn_exp2f(fmaf(s[w / 8][2 * w % 16], c1, -sub));
             const float b2 = __builtin_amdgcn_exp2f(fmaf(s[w / 8][2 * w % 16 + 1], c1, -sub));
-            sum += a + b2;
             p[w] = T::pack(a, b2);
+            sum = T::add(p[w], sum);                        // as rounded: a row of few keys then divides the rounding out
           }
         }
         if (j >= NQK - LV) vr[j - (NQK - LV)] = read_v(va, j - (NQK - LV));

@@ -18,6 +18,10 @@ template <> struct GmT16<GM_QTYPE_BF16> {
     V2 v = {(__bf16)a, (__bf16)b};
     return __builtin_bit_cast(uint32_t, v);
   }
+  // c + both elements
+  static __device__ __forceinline__ float add(uint32_t w, float c) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(V2, w), __builtin_bit_cast(V2, 0x3f803f80u), c, false);
+  }
   static __device__ __forceinline__ gm_f32x4 mfma16(gm_u32x4 a, gm_u32x4 b, gm_f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
   }
@@ -33,6 +37,9 @@ template <> struct GmT16<GM_QTYPE_F16> {
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     V2 v = {(_Float16)a, (_Float16)b};
     return __builtin_bit_cast(uint32_t, v);
+  }
+  static __device__ __forceinline__ float add(uint32_t w, float c) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(V2, w), __builtin_bit_cast(V2, 0x3c003c00u), c, false);
   }
   static __device__ __forceinline__ gm_f32x4 mfma16(gm_u32x4 a, gm_u32x4 b, gm_f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), c, 0, 0, 0);
