@@ -32,7 +32,7 @@
 //
 // Bound: MFMA, with the exponentials beside them; for short prompts the latency of a
 // block's first loads and its epilogue.  Measured: 16,000 tokens of 16 heads of 256 on 2,
-// bf16, 2.32 ms (900 TFLOP/s of the 1,110 of a large product); 8,192 tokens in 11 prompts,
+// bf16, 2.29 ms (915 TFLOP/s of the 1,110 of a large product); 8,192 tokens in 11 prompts,
 // 32 heads of 128 on 8, fp16, 136 us (675); 301 tokens in 5, 16 of 256, 30 us.  With a
 // running maximum and the rescaling the first took 15.6 ms, its registers spilled.
 #include "kernels.h"
